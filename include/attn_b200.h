@@ -38,7 +38,8 @@ extern "C" {
 #define ATTN_B200_DTYPE_FP16 0
 #define ATTN_B200_DTYPE_BF16 1
 #define ATTN_B200_DTYPE_SAME 0         /* dtype_out: the output has the dtype of the inputs */
-#define ATTN_B200_DTYPE_FP32 2         /* dtype_out: fp32 output (accumulators stored unrounded) */
+#define ATTN_B200_DTYPE_FP32 2         /* dtype_out: fp32 output (accumulators stored unrounded); rotary: fp32 operands */
+#define ATTN_B200_DTYPE_E4M3 3         /* paged caches: 8-bit codes (1-4-3, no infinities) with a scale for each token and head */
 
 #define ATTN_B200_MASK_NONE 0
 #define ATTN_B200_MASK_CAUSAL 1        /* keep q_idx >= kv_idx (top-left aligned)           */
@@ -406,6 +407,117 @@ typedef struct AttnB200ElementwiseBwdArgs {
   const void* mask_tiles_q;
   const void* mask_tiles_kv;
 } AttnB200ElementwiseBwdArgs;
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * Rotary positions and paged caches of softmax attention (no counterpart in the reference; they stand beside its paged MLA
+ * decode, core/template/cute_template_kvshared/flash_api.cpp:61-210).
+ * ------------------------------------------------------------------------------------------------------------------ */
+
+/* How the first `dim` columns of a head turn with the position: pair i by the angle position * turns[i] / 2^64 of a full
+ * turn, (a, b) -> magnitude * (a cos - b sin, b cos + a sin).  turns is a 64-bit fraction, so that the product wraps at whole
+ * turns and the angle of a far position is as exact as that of a near one. */
+typedef struct AttnB200Rotary {
+  const uint64_t* turns;   /* device, [dim / 2] */
+  int32_t dim;             /* even, at most the head dim; 0 = nothing turns */
+  int32_t interleaved;     /* pairs (2 i, 2 i + 1) instead of (i, i + dim / 2) */
+  float magnitude;
+  int32_t reserved;
+} AttnB200Rotary;
+
+/* y = x with its heads turned, for one tensor or for q and k together (x[1] NULL = one).  [batch, seq, heads, head_dim] as
+ * seen through the element strides, last dimension contiguous; y may be x with the same strides, and overlaps nothing else. */
+typedef struct AttnB200RotaryArgs {
+  const void* x[2];
+  void* y[2];
+  const void* positions;       /* int32 or int64 through pos_stride, or NULL: 0, 1, ... along seq */
+  int64_t x_stride[2][3];      /* (batch, seq, head) */
+  int64_t y_stride[2][3];
+  int64_t pos_stride[2];       /* (batch, seq) */
+  int32_t heads[2];
+  int32_t batch, seq, head_dim;
+  int32_t dtype;               /* ATTN_B200_DTYPE_FP16, _BF16 or _FP32 */
+  int32_t positions_64;        /* 1: positions are int64 */
+  int32_t inverse;             /* 1: by the opposite angle (the backward pass: the transposed map) */
+  AttnB200Rotary rotary;
+} AttnB200RotaryArgs;
+
+int attn_b200_rotary(const AttnB200RotaryArgs* args, void* cuda_stream);
+
+/* A cache of keys and values in pages, and the sequences of a call: token t of sequence b lies in row t % page_size of page
+ * block_table[b][t / page_size].  Entries at and behind a sequence's end are not looked at; one inside it that names no page
+ * reads as zeros and is not written. */
+typedef struct AttnB200PagedCache {
+  void* k;                     /* [num_pages, page_size, heads_kv, head_dim] through the strides, last dimension contiguous */
+  void* v;
+  uint8_t* k_scale;            /* E4M3: [num_pages, page_size, heads_kv] exponents e; a code stands for code * 2^(e - 127), 255 for NaN */
+  uint8_t* v_scale;
+  int64_t k_stride[3];         /* elements of (page, token, head) */
+  int64_t v_stride[3];
+  int64_t k_scale_stride[3];
+  int64_t v_scale_stride[3];
+  const int32_t* block_table;  /* [batch][max_blocks], rows block_table_stride apart */
+  int64_t block_table_stride;
+  const int32_t* seq_lens;     /* [batch] tokens of each sequence, the new ones among them; at most max_blocks * page_size count */
+  int32_t num_pages, page_size, heads_kv, head_dim, max_blocks, batch;
+  int32_t dtype;               /* ATTN_B200_DTYPE_FP16, _BF16 or _E4M3 */
+  int32_t reserved;
+} AttnB200PagedCache;
+
+/* Writes the last tokens of each sequence into the cache.  k, v: [batch, seq, heads_kv, head_dim], or with cu_seqlens
+ * (int32 [batch + 1]) packed rows [seq, heads_kv, head_dim] of which cu_seqlens[b] .. cu_seqlens[b + 1] - 1 are the last
+ * tokens of sequence b; rows behind cu_seqlens[batch] and tokens at negative positions go nowhere.  E4M3: the scale of a
+ * row is the least power of two (from 2^-127) that brings its largest magnitude to 448 at most; a row with a value that is
+ * not finite is NaN throughout.  `rotary` turns k on its way, in 32 bits and rounded once. */
+typedef struct AttnB200PagedAppendArgs {
+  AttnB200PagedCache cache;
+  const void* k;
+  const void* v;
+  const int32_t* cu_seqlens;
+  int64_t k_stride[3];         /* (batch, seq, head); packed: the first is not looked at */
+  int64_t v_stride[3];
+  int32_t seq;
+  int32_t dtype;               /* of k and v: FP16 or BF16, the cache's own unless that is E4M3 */
+  AttnB200Rotary rotary;       /* dim a multiple of 16, or 0 */
+} AttnB200PagedAppendArgs;
+
+int attn_b200_paged_append(const AttnB200PagedAppendArgs* args, void* cuda_stream);
+
+/* Reads the cache back: contiguous k, v [batch, max_len, heads_kv, head_dim] in FP16 or BF16, zeros behind the ends. */
+typedef struct AttnB200PagedReadArgs {
+  AttnB200PagedCache cache;
+  void* k;
+  void* v;
+  int32_t max_len;
+  int32_t dtype;
+} AttnB200PagedReadArgs;
+
+int attn_b200_paged_read(const AttnB200PagedReadArgs* args, void* cuda_stream);
+
+/* Attention of the new tokens of each sequence over what its pages hold, softmax(scale * Q.K^T).V with grouped heads: row at
+ * position p (the new tokens are the last ones) sees the keys at p and in front of it (causal = 1; 0: all), with window > 0
+ * only those from p - window + 1 on.  A row that sees none gives 0 and -inf.  q, o: [batch, seq, heads, head_dim], or with
+ * cu_seqlens packed rows [seq, heads, head_dim] as in AttnB200PagedAppendArgs; packed rows behind cu_seqlens[batch] are left
+ * as they are.  An 8-bit cache is read as the 16-bit values of q's type that its codes stand for.  At most 1024 sequences,
+ * 128 query heads to a KV head. */
+typedef struct AttnB200PagedAttnArgs {
+  AttnB200PagedCache cache;
+  const void* q;
+  void* o;
+  float* lse;                  /* [batch, heads, seq], packed [heads, seq]; or NULL */
+  const int32_t* cu_seqlens;
+  int64_t q_stride[3];         /* elements of (batch, seq, head); packed: the first is not looked at */
+  int64_t o_stride[3];
+  int32_t heads, seq;
+  int32_t dtype;               /* of q and o: FP16 or BF16, the cache's own unless that is E4M3 */
+  float scale;                 /* > 0 */
+  int32_t causal, window;
+  void* workspace;             /* attn_b200_paged_workspace_bytes() bytes of device scratch, 16-byte aligned */
+  int64_t workspace_bytes;
+} AttnB200PagedAttnArgs;
+
+/* Scratch of a call; -1 = arguments that attn_b200_paged_attention does not take.  Looks at no device memory. */
+int64_t attn_b200_paged_workspace_bytes(const AttnB200PagedAttnArgs* args);
+int attn_b200_paged_attention(const AttnB200PagedAttnArgs* args, void* cuda_stream);
 
 /* Reads and clears the device-side status word of device `device`
  * (0 = no kernel reported a problem).  Synchronises the device. */

@@ -17,8 +17,8 @@ if _here not in _sys.path:
 
 __version__ = "0.1.0"
 
-from attn_engine import AttentionEngine, LinearAttentionEngine, OnlineFunc  # noqa: E402
+from attn_engine import AttentionEngine, LinearAttentionEngine, OnlineFunc, PagedKVCache, RotaryEmbedding  # noqa: E402
 from core import CustomIO, SymbolicArray, SymbolicTensor, SymbolScalar, Var, meta_tensor  # noqa: E402
 
 __all__ = ["AttentionEngine", "LinearAttentionEngine", "OnlineFunc", "CustomIO", "SymbolicArray",
-           "SymbolicTensor", "SymbolScalar", "Var", "meta_tensor"]
+           "SymbolicTensor", "SymbolScalar", "Var", "meta_tensor", "PagedKVCache", "RotaryEmbedding"]

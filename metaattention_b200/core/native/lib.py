@@ -138,6 +138,46 @@ class MlaArgs(C.Structure):
     ]
 
 
+class Rotary(C.Structure):
+    _fields_ = [("turns", C.c_void_p), ("dim", C.c_int32), ("interleaved", C.c_int32), ("magnitude", C.c_float), ("reserved", C.c_int32)]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p * 2), ("y", C.c_void_p * 2), ("positions", C.c_void_p),
+        ("x_stride", (C.c_int64 * 3) * 2), ("y_stride", (C.c_int64 * 3) * 2), ("pos_stride", C.c_int64 * 2), ("heads", C.c_int32 * 2),
+        ("batch", C.c_int32), ("seq", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32), ("positions_64", C.c_int32), ("inverse", C.c_int32),
+        ("rotary", Rotary),
+    ]
+
+
+class PagedCacheArgs(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("k_scale_stride", C.c_int64 * 3), ("v_scale_stride", C.c_int64 * 3),
+        ("block_table", C.c_void_p), ("block_table_stride", C.c_int64), ("seq_lens", C.c_void_p),
+        ("num_pages", C.c_int32), ("page_size", C.c_int32), ("heads_kv", C.c_int32), ("head_dim", C.c_int32), ("max_blocks", C.c_int32),
+        ("batch", C.c_int32), ("dtype", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [("cache", PagedCacheArgs), ("k", C.c_void_p), ("v", C.c_void_p), ("cu_seqlens", C.c_void_p),
+                ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("seq", C.c_int32), ("dtype", C.c_int32), ("rotary", Rotary)]
+
+
+class PagedReadArgs(C.Structure):
+    _fields_ = [("cache", PagedCacheArgs), ("k", C.c_void_p), ("v", C.c_void_p), ("max_len", C.c_int32), ("dtype", C.c_int32)]
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCacheArgs), ("q", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p), ("cu_seqlens", C.c_void_p),
+        ("q_stride", C.c_int64 * 3), ("o_stride", C.c_int64 * 3), ("heads", C.c_int32), ("seq", C.c_int32), ("dtype", C.c_int32),
+        ("scale", C.c_float), ("causal", C.c_int32), ("window", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
 # symbol name -> (restype, argtypes); must list every function of include/attn_b200.h
 SIGNATURES = {
     "attn_b200_parallel_fwd": (C.c_int, [C.POINTER(ParallelArgs), C.c_void_p]),
@@ -162,6 +202,11 @@ SIGNATURES = {
     "attn_b200_mla_metadata": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]),
     "attn_b200_mla_decode": (C.c_int, [C.POINTER(MlaArgs), C.c_void_p]),
     "attn_b200_mla_decode_static": (C.c_int, [C.POINTER(MlaArgs), C.c_void_p, C.c_void_p]),
+    "attn_b200_rotary": (C.c_int, [C.POINTER(RotaryArgs), C.c_void_p]),
+    "attn_b200_paged_append": (C.c_int, [C.POINTER(PagedAppendArgs), C.c_void_p]),
+    "attn_b200_paged_read": (C.c_int, [C.POINTER(PagedReadArgs), C.c_void_p]),
+    "attn_b200_paged_workspace_bytes": (C.c_int64, [C.POINTER(PagedAttnArgs)]),
+    "attn_b200_paged_attention": (C.c_int, [C.POINTER(PagedAttnArgs), C.c_void_p]),
     "attn_b200_last_device_status": (C.c_int, [C.c_int32, C.POINTER(C.c_int32)]),
     "attn_b200_device_status_word": (C.c_int, [C.c_int32, C.POINTER(C.c_void_p)]),
     "attn_b200_version": (C.c_int, []),
@@ -171,7 +216,8 @@ _lib = None
 
 
 def library_sources() -> list[str]:
-    return [os.path.join(CSRC_DIR, f) for f in ("attn_b200.cu", "decode_fwd.cu", "mla_decode.cu", "linear_fwd.cu", "softmax_bwd.cu", "row_ops.cu")]
+    return [os.path.join(CSRC_DIR, f) for f in ("attn_b200.cu", "decode_fwd.cu", "mla_decode.cu", "linear_fwd.cu", "softmax_bwd.cu", "row_ops.cu", "rotary.cu",
+                                               "paged_ops.cu", "paged_attention.cu")]
 
 
 def build_library(force: bool = False, verbose: bool = False) -> str:
@@ -211,7 +257,7 @@ def host_path() -> str:
     """Where the native host side lies that belongs to these sources and this torch: it fills the structs of the header by
     their compiled-in layout and calls torch's C++ API, so one built from others is never loaded."""
     key = hashlib.sha256(" ".join([torch.__version__, *HOST_FLAGS]).encode())
-    for path in (os.path.join(CSRC_DIR, "host_ops.cpp"), os.path.join(INCLUDE_DIR, "attn_b200.h")):
+    for path in (os.path.join(CSRC_DIR, "host_ops.cpp"), os.path.join(CSRC_DIR, "paged_host.h"), os.path.join(INCLUDE_DIR, "attn_b200.h")):
         with open(path, "rb") as f:
             key.update(f.read())
     return os.path.join(_PKG_DIR, f"_host_ops_{key.hexdigest()[:16]}.so")

@@ -19,9 +19,11 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <map>
 #include <memory>
+#include <sstream>
 #include <tuple>
 
 #include "../../include/attn_b200.h"
@@ -879,11 +881,17 @@ py::object mla_decode_call(const Tensor& q, const Tensor& kv, int64_t dim_v, dou
   return py::make_tuple(r.o, r.lse, r.num_splits, r.parts);
 }
 
+#include "paged_host.h"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   py::class_<Plan, std::shared_ptr<Plan>>(m, "Plan");
-  m.def("bind", &bind);
+  m.def("bind", [](const py::dict& d, py::object check) {
+    bind(d, check);
+    bind_paged(d);
+  });
+  def_paged(m);
   m.def("make_plan", &make_plan);
   m.def("run", &run);
   m.def("softmax_bwd", &softmax_bwd_call);
