@@ -217,7 +217,7 @@ _lib = None
 
 def library_sources() -> list[str]:
     return [os.path.join(CSRC_DIR, f) for f in ("attn_b200.cu", "decode_fwd.cu", "mla_decode.cu", "linear_fwd.cu", "softmax_bwd.cu", "row_ops.cu", "rotary.cu",
-                                               "paged_ops.cu", "paged_attention.cu")]
+                                               "paged_ops.cu", "paged_attention.cu", "paged_tokens.cu", "paged_chunk.cu")]
 
 
 def build_library(force: bool = False, verbose: bool = False) -> str:

@@ -162,12 +162,10 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p)
         for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
 #pragma unroll
         for (int d = 1; d < kUnits; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-        // top = m 2^(E - 127), 1 <= m < 2: the least e with m 2^(E - 127 - e) <= 448 = 1.75 * 2^8
         const bool finite = top < 0x7f800000u;
-        int e = static_cast<int>(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-        e = max(e, -127);
+        const int e = max(code_exponent(top), -127);
         const int byte = finite ? e + 127 : 255;
-        const float inv = __uint_as_float(e <= 126 ? static_cast<uint32_t>(127 - e) << 23 : 0x00400000u);   // 2^-e, exact; e is at most 120
+        const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);   // 2^-e; e is at most 121
         if (on) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] = finite ? x[i] * inv : __uint_as_float(0x7fffffffu);

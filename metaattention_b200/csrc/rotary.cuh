@@ -1,5 +1,6 @@
 // Rotary positions: the angle of a pair of columns and the turned values, for the kernels that turn q and k (rotary.cu) and
-// the one that turns k on its way into a cache (paged_ops.cu).
+// the one that turns k on its way into a cache (paged_ops.cu).  And the scale of a row of 8-bit codes, for the latter and for
+// attention over such caches (paged_attention.cu).
 #pragma once
 
 #include "../../include/attn_b200.h"
@@ -37,6 +38,11 @@ template <bool kBf16>
 __device__ __forceinline__ float2 unpack2(uint32_t w) {
   if constexpr (kBf16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
   else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// The least e with a value of these bits (without sign) <= 448 * 2^e = 1.75 * 2^(8 + e); down to -127 - 8 for zero.
+__device__ __forceinline__ int code_exponent(uint32_t top) {
+  return static_cast<int>(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
 }
 
 }  // namespace b200
