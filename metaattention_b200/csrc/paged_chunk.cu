@@ -16,14 +16,14 @@ struct PagedSmem {
   static constexpr int kKBytes = k8Bit ? kRawBytes : kTileBytes;
   static constexpr int kStagesK = k8Bit ? (D == 128 ? 4 : 8) : D == 128 ? 3 : 6, kStagesV = k8Bit ? 2 : D == 128 ? 2 : 5;
   static constexpr int kRaw = k8Bit ? (D == 128 ? (kBf16 ? 3 : 2) : 6) : 0;   // tiles of codes of V
-  static constexpr int kScales = k8Bit ? 4 : 0;                     // tiles of exponents
+  static constexpr int kScales = k8Bit ? 4 : 0;                      // tiles of exponents
   // query tiles; an MMA reads 128 rows from a tile's start whatever its rows, so what follows must be shared memory too
   static constexpr int kQRegion = k8Bit ? kPieces * kRawBytes : D * 256;
   static constexpr int kOffK = kQRegion;
   static constexpr int kOffV = kOffK + kStagesK * kKBytes;
   static constexpr int kOffRaw = kOffV + kStagesV * kTileBytes;
   static constexpr int kOffScales = kOffRaw + kRaw * kRawBytes;     // uint8 [kScales][2][128]
-  static constexpr int kOffQs = kOffScales + kScales * 2 * kPgTile; // float [4][128]: factors of the query rows, by unit
+  static constexpr int kOffQs = kOffScales + kScales * 2 * kPgTile;   // float [4][128]: factors of the query rows, by unit
   static constexpr int kOffBar = kOffQs + (k8Bit ? 4 * kPgTile * 4 : 0);
   static constexpr int kQFull = 0, kQEmpty = 2, kSFull = 4, kPReady = 6, kODone = 8, kStats = 10, kOFree = 11, kKFull = 12;
   static constexpr int kKEmpty = kKFull + kStagesK, kVFull = kKEmpty + kStagesK, kVEmpty = kVFull + kStagesV;
@@ -189,11 +189,9 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
           if (i == 0 && ui > 0) ok = wait(bars + L::kOFree, (ui - 1) & 1, kPgOFree);   // the accumulators have been read
           ok = ok && wait(bars + L::kVFull + st, (J / L::kStagesV) & 1, kPgVFull);
           if (!ok) break;
-          if constexpr (!k8Bit) {
-            int a, e;
-            u.rows_of(i, a, e);
-            if (a > 0 || e < N) paged_zero_rows<KC>(sV + st * L::kTileBytes, a, e);
-          }
+          int a, e;
+          u.rows_of(i, a, e);
+          if (a > 0 || e < N) paged_zero_rows<KC>(sV + st * L::kTileBytes, a, e);
           ok = wait(bars + L::kPReady + t, (J >> 1) & 1, kPgPReady);
           if (!ok) break;
           tc_fence_after_sync();
@@ -461,13 +459,11 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
         if (more && p.q_bufs == 2) ok = split(ui + 1);   // else when the unit's last scores are under way
         for (int i = 0; i < u.n && ok; ++i, ++J) {
           const int sc = J % L::kScales, raw = J % L::kRaw, st = J % L::kStagesV;
-          ok = warp_all(mbar_wait(bars + L::kScFull + sc, (J / L::kScales) & 1, ab, kPgScales));
-          ok = ok && warp_all(mbar_wait(bars + L::kRawFull + raw, (J / L::kRaw) & 1, ab, kPgRawFull));
-          ok = ok && warp_all(mbar_wait(bars + L::kVEmpty + st, ((J / L::kStagesV) & 1) ^ 1, ab, kPgVEmpty));
+          ok = warp_all(paged_wait(bars + L::kScFull + sc, (J / L::kScales) & 1, ab, kPgScales));
+          ok = ok && warp_all(paged_wait(bars + L::kRawFull + raw, (J / L::kRaw) & 1, ab, kPgRawFull));
+          ok = ok && warp_all(paged_wait(bars + L::kVEmpty + st, ((J / L::kStagesV) & 1) ^ 1, ab, kPgVEmpty));
           if (!ok) break;
-          int a, e;
-          u.rows_of(i, a, e);
-          paged_widen<D, kBf16, kPgConvWarps>(smem + L::kOffRaw + raw * L::kRawBytes, smem + L::kOffScales + (sc * 2 + 1) * N, sV + st * L::kTileBytes, ct, a, e);
+          paged_widen<D, kBf16, kPgConvWarps>(smem + L::kOffRaw + raw * L::kRawBytes, smem + L::kOffScales + (sc * 2 + 1) * N, sV + st * L::kTileBytes, ct);
           if (lane == 0) {
             mbar_arrive(bars + L::kVFull + st);
             mbar_arrive(bars + L::kRawEmpty + raw);

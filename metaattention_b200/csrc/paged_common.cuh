@@ -58,6 +58,15 @@ enum PagedWaitSite {
   kPgScales, kPgScalesEmpty, kPgSFree, kPgSmemAlign
 };
 
+// mbar_wait() whose way out of line is a call: most waits end in their first attempt, which the hardware suspends, and where
+// twenty warps run seven different loops every instruction in line counts.
+static __device__ __noinline__ bool paged_wait_on(uint64_t* bar, uint32_t parity, volatile int* cta_flag, int* status, int site) {
+  return mbar_wait(bar, parity, AbortState{cta_flag, status}, site);
+}
+__device__ __forceinline__ bool paged_wait(uint64_t* bar, uint32_t parity, const AbortState& ab, int site) {
+  return mbar_try_wait(bar, parity) || paged_wait_on(bar, parity, ab.cta_flag, ab.device_status, site);
+}
+
 __host__ __device__ __forceinline__ int pg_share(int total, int c, int n) { return static_cast<int>(static_cast<long long>(total) * c / n); }
 __device__ __forceinline__ int pg_owner(int t, int n, int total) { return static_cast<int>((static_cast<long long>(t + 1) * n - 1) / total); }
 
@@ -250,7 +259,7 @@ __device__ __forceinline__ void paged_load(const PagedParams& p, PagedWalk u, co
       const bool mine = blk < bpt && blk * box < e && (blk + 1) * box > a;
       const int boxes = e > a ? (e + box - 1) / box - a / box : 0;
       const int row = ((u.lo + u.t0 + i) * kPgTile + blk * box) & ((1 << p.page_shift) - 1);
-      if (!warp_all(mbar_wait(empty + st, par, ab, site))) return;
+      if (!warp_all(paged_wait(empty + st, par, ab, site))) return;
       if (lane == 0) mbar_arrive_expect_tx(full + st, boxes * box * kParts * kRowBytes);
       __syncwarp();
       // a page that does not exist is out of the map's bounds: zeros
@@ -318,8 +327,8 @@ __device__ __forceinline__ float key_factor(int byte) {
 }
 
 // 8-bit caches: a warp that brings the rows' exponents, of K and of V, into a ring of slots [2][128]; a lane four rows of each,
-// copied without waiting.  (Four tiles of them in registers, turned into factors here, were the bound of the whole kernel:
-// 3800 to 6000 cycles a tile.  Who uses a factor makes it.)  `full` counts 32 arrivals.  A page that does not exist gives zeros.
+// copied without waiting; who uses a factor makes it.  (Made here they were the bound of the whole kernel: 3800 to 6000 cycles a
+// tile with the exponents in registers, 2100 behind copies.)  `full` counts 32 arrivals.  A page that does not exist gives zeros.
 template <int kSlots>
 __device__ __forceinline__ void paged_scales(const PagedParams& p, PagedWalk u, uint8_t* ring, uint64_t* full, uint64_t* empty, const AbortState& ab) {
   const int lane = threadIdx.x & 31;
@@ -340,7 +349,7 @@ __device__ __forceinline__ void paged_scales(const PagedParams& p, PagedWalk u, 
       const int after = page_at(i + 2);
       const bool there = page >= 0 && page < p.pages;
       const int row = ((u.lo + u.t0 + i) * kPgTile + 4 * lane) & ((1 << p.page_shift) - 1);
-      if (!warp_all(mbar_wait(empty + st, par, ab, kPgScalesEmpty))) return;
+      if (!warp_all(paged_wait(empty + st, par, ab, kPgScalesEmpty))) return;
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
         const uint8_t* s = p.scale8[kv] + (there ? page * p.scale_stride[kv][0] + row * p.scale_stride[kv][1] + u.h * p.scale_stride[kv][2] : 0);
@@ -420,23 +429,21 @@ __device__ __forceinline__ void paged_split_queries(const PagedParams& p, const 
   __syncwarp();
 }
 
-// A tile of V from codes to 16 bits, by kWarps warps: chunks of 128-byte rows, swizzled as TMA would have written them.  Rows
-// outside [a, e) become zeros.
+// A tile of V from codes to 16 bits, by kWarps warps: chunks of 128-byte rows, swizzled as TMA would have written them.
 template <int D, bool kBf16, int kWarps>
-__device__ __forceinline__ void paged_widen(const uint8_t* src, const uint8_t* exponents, uint8_t* dst, int ct, int a, int e) {
+__device__ __forceinline__ void paged_widen(const uint8_t* src, const uint8_t* exponents, uint8_t* dst, int ct) {
   constexpr int kUnits = D / 16, kStep = 32 * kWarps / kUnits;   // pieces of 16 columns of a row, rows at a time
-  constexpr uint32_t kOne = kBf16 ? 0x3f80u : 0x3c00u;
   const int unit = ct % kUnits;
   // columns 16 unit to + 15 are two 16-byte pieces of the row's chunk
   const int piece = (unit % 4) * 2, swap = (unit / 4) & 1;
   dst += unit / 4 * (kPgTile * 128);
   // Not unrolled: several roles share a scheduler's instruction cache, and straight code that runs once a tile comes from behind
   // it (unrolled by four 2000 cycles a tile, 40 % of all stalls on instructions).  The next piece is on its way meanwhile.
-  const uint32_t at = smem_u32(src) + unit * 16, exp_at = smem_u32(exponents);
+  const uint32_t at = smem_u32(src) + unit * 16, exponent_at = smem_u32(exponents);
   auto load_exponent = [&](int row) {
     uint32_t x;
-    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(x) : "r"(exp_at + row) : "memory");
-    return static_cast<int>(x);
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(x) : "r"(exponent_at + row) : "memory");
+    return x;
   };
   // half of the threads begin with the second half of their piece, so that eight neighbours write to all banks
   auto load_codes = [&](int row, int half) {
@@ -446,35 +453,31 @@ __device__ __forceinline__ void paged_widen(const uint8_t* src, const uint8_t* e
   };
   int row = ct / kUnits;
   uint2 c0 = load_codes(row, 0), c1 = load_codes(row, 1);
-  int byte = load_exponent(row);
+  uint32_t byte = load_exponent(row);
   const uint32_t line = smem_u32(dst);
 #pragma unroll 1
   while (row < kPgTile) {
     const int next = min(row + kStep, kPgTile - 1);
     const uint2 c0_next = load_codes(next, 0), c1_next = load_codes(next, 1);
-    const int byte_next = load_exponent(next);
-    const bool in = row >= a && row < e;
-    // 2^(byte - 127) times what widen4() leaves out
-    uint32_t f1 = kBf16 ? (byte + 120) << 7 : (byte - 104) << 10, f2 = kOne;
-    if (kBf16 ? byte > 134 : static_cast<uint32_t>(byte - 105) > 29u) {   // outside the format: rows of very large or small values
-      const uint32_t f = row_factor<kBf16>(byte);
-      f1 = f & 0xffffu;
-      f2 = f >> 16;
-    }
-    f1 = in ? f1 * 0x10001u : 0u;
+    const uint32_t byte_next = load_exponent(next);
     const uint32_t c4[4] = {c0.x, c0.y, c1.x, c1.y};
     uint32_t w[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const uint2 x = widen4<kBf16>(c4[k]);
-      w[2 * k] = mul2<kBf16>(x.x, f1);
-      w[2 * k + 1] = mul2<kBf16>(x.y, f1);
+      w[2 * k] = x.x;
+      w[2 * k + 1] = x.y;
     }
-    if (f2 != kOne) {
-      const uint32_t ff = in ? f2 * 0x10001u : 0u;
+    // 2^(byte - 127) times what widen4() leaves out, in both halves of a word
+    uint32_t factor = kBf16 ? (byte + 120u) * 0x00800080u : (byte - 104u) * 0x04000400u;
+    if (kBf16 ? byte > 134u : byte - 105u > 29u) {   // not a 16-bit power of two: rows of very large or very small values
+      const uint32_t f = row_factor<kBf16>(byte);
+      factor = __byte_perm(f, 0, 0x1010);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) w[k] = mul2<kBf16>(w[k], ff);
+      for (int k = 0; k < 8; ++k) w[k] = mul2<kBf16>(w[k], __byte_perm(f, 0, 0x3232));
     }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = mul2<kBf16>(w[k], factor);
     const uint32_t p0 = (piece + swap) ^ (row & 7);
     st_shared_v4(line + row * 128 + p0 * 16, make_uint4(w[0], w[1], w[2], w[3]));
     st_shared_v4(line + row * 128 + (p0 ^ 1) * 16, make_uint4(w[4], w[5], w[6], w[7]));

@@ -40,7 +40,7 @@ struct TokensSmem {
   static constexpr int kOffV = kOffK + kStagesK * kKBytes;
   static constexpr int kOffRaw = kOffV + kStagesV * kTileBytes;
   static constexpr int kOffScales = kOffRaw + kRaw * kRawBytes;      // uint8 [kScales][2][128]
-  static constexpr int kOffQs = kOffScales + kScales * 2 * kPgTile;  // float [4][R]: factors of the query rows, by unit
+  static constexpr int kOffQs = kOffScales + kScales * 2 * kPgTile;   // float [4][R]: factors of the query rows, by unit
   // float [2][2][R] by unit and group: reference maxima, and sums; float [2][R] by group: rescales; int [R]: positions in the tile
   static constexpr int kOffRow = kOffQs + (k8Bit ? 4 * R * 4 : 0);
   static constexpr int kOffWarp = kOffRow + 11 * R * 4;              // float [8][R]: a value of each warp
@@ -158,7 +158,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
                                                            [&](const PagedWalk& u, int ui) -> bool {
       if constexpr (!k8Bit) {
         const int qb = ui & 1;
-        if (ui >= 2 && !warp_all(mbar_wait(bars + L::kQEmpty + qb, ((ui >> 1) - 1) & 1, ab, kPgQEmpty))) return false;
+        if (ui >= 2 && !warp_all(paged_wait(bars + L::kQEmpty + qb, ((ui >> 1) - 1) & 1, ab, kPgQEmpty))) return false;
         if (lane == 0) {
           mbar_arrive_expect_tx(bars + L::kQFull + qb, KC * p.rows * 128);
           const int s = p.cu != nullptr ? tab.row[u.b] + u.qt * p.per_tile : u.qt * p.per_tile;
@@ -178,7 +178,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
                                        [](const PagedWalk&, int) { return true; });
   } else if (warp == 10) {
     // ======================= issues S^T = K Q^T (converged, one elected lane a batch) =======================
-    auto wait = [&](uint64_t* bar, uint32_t parity, int site) -> bool { return warp_all(k8Bit ? mbar_wait(bar, parity, ab, site) : mbar_wait_poll(bar, parity, ab, site)); };
+    auto wait = [&](uint64_t* bar, uint32_t parity, int site) -> bool { return warp_all(k8Bit ? paged_wait(bar, parity, ab, site) : mbar_wait_poll(bar, parity, ab, site)); };
     auto operand = [](uint32_t at) { return k8Bit && D == 64 ? make_smem_desc_64b(at) : make_smem_desc(at, 16, 1024); };
     const uint64_t k_desc0 = operand(smem_u32(sK)), q_desc0 = operand(smem_u32(sQ));
     PagedWalk u = make_walk();
@@ -218,7 +218,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
     }
   } else if (warp == 11) {
     // ======================= issues O^T += V^T P =======================
-    auto wait = [&](uint64_t* bar, uint32_t parity, int site) -> bool { return warp_all(k8Bit ? mbar_wait(bar, parity, ab, site) : mbar_wait_poll(bar, parity, ab, site)); };
+    auto wait = [&](uint64_t* bar, uint32_t parity, int site) -> bool { return warp_all(k8Bit ? paged_wait(bar, parity, ab, site) : mbar_wait_poll(bar, parity, ab, site)); };
     // V [key][column] is V^T with the columns as rows, M-major; 64 columns are given twice (the same chunk again), their second
     // results are not looked at
     const uint64_t v_desc0 = make_smem_desc(smem_u32(sV), D == 128 ? kChunk : 0, 1024);
@@ -233,11 +233,9 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
       for (int i = 0; i < u.n && ok; ++i, ++J) {
         ok = wait(bars + L::kVFull + st, par, kPgVFull);
         if (!ok) break;
-        if constexpr (!k8Bit) {   // (codes are widened with a factor of zero there)
-          int a, e;
-          u.rows_of(i, a, e);
-          if (a > 0 || e < N) paged_zero_rows<KC>(sV + st * L::kTileBytes, a, e);
-        }
+        int a, e;
+        u.rows_of(i, a, e);
+        if (a > 0 || e < N) paged_zero_rows<KC>(sV + st * L::kTileBytes, a, e);
         ok = wait(bars + L::kPReady + (J & 1), (J >> 1) & 1, kPgPReady);
         if (!ok) break;
         tc_fence_after_sync();
@@ -286,7 +284,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
       for (int r = 0; r < R; ++r) acc[r] = 0.0f;
       for (int i = (J0 ^ group) & 1; i < u.n; i += 2) {
         const int J = J0 + i, sb = J % L::kScores;
-        mbar_wait_rows(bars + L::kSFull + sb, (J / L::kScores) & 1, ab, kPgSFull);
+        paged_wait(bars + L::kSFull + sb, (J / L::kScores) & 1, ab, kPgSFull);
         tc_fence_after_sync();
         float s[R];
         load_rows(tS + sb * R, s);
@@ -296,11 +294,12 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
         if (lane == 0) mbar_arrive(bars + L::kSFree + sb);
         if constexpr (k8Bit) {
           const int slot = J % L::kScales;
-          mbar_wait_rows(bars + L::kScFull + slot, (J / L::kScales) & 1, ab, kPgScales);
+          paged_wait(bars + L::kScFull + slot, (J / L::kScales) & 1, ab, kPgScales);
           const float f = key_factor(smem[L::kOffScales + slot * 2 * N + key0]) * c2;
           const float4* qs = reinterpret_cast<const float4*>(smem + L::kOffQs) + (ui & 3) * (R / 4);
 #pragma unroll
           for (int r = 0; r < R; r += 4) {
+            if (r >= p.rows) break;
             const float4 q = qs[r / 4];
             s[r] *= f * q.x;
             s[r + 1] *= f * q.y;
@@ -311,12 +310,16 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
           if (lane == 0) mbar_arrive(bars + L::kScEmpty + slot);
         } else {
 #pragma unroll
-          for (int r = 0; r < R; ++r) s[r] *= c2;
+          for (int r = 0; r < R; ++r) {
+            if (r % 4 == 0 && r >= p.rows) break;
+            s[r] *= c2;
+          }
         }
         const int kv0 = (u.lo + u.t0 + i) * N, key = kv0 + key0;
         if (kv0 < all_begin || kv0 + N > all_end) {
 #pragma unroll
           for (int r = 0; r < R; ++r) {
+            if (r % 4 == 0 && r >= p.rows) break;
             const int pos = first + s_pos[r];
             const bool in = key < u.end && (!p.causal || key <= pos) && (p.window == 0 || key > pos - p.window);
             s[r] = in ? s[r] : -INFINITY;
@@ -325,6 +328,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
         float ref[R], over = -INFINITY;
 #pragma unroll
         for (int r = 0; r < R; r += 4) {
+          if (r >= p.rows) break;
           const float4 m = reinterpret_cast<const float4*>(s_ref)[r / 4];
           ref[r] = m.x;
           ref[r + 1] = m.y;
@@ -338,6 +342,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
           float mine = 0.0f;
 #pragma unroll
           for (int r = 0; r < R; ++r) {
+            if (r % 4 == 0 && r >= p.rows) break;
             const float m = warp_max(s[r]);
             if (lane == r) mine = m;
           }
@@ -353,14 +358,18 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
           float scale[R];
 #pragma unroll
           for (int r = 0; r < R; r += 4) {
+            if (r >= p.rows) break;
             const float4 m = reinterpret_cast<const float4*>(s_ref)[r / 4], x = reinterpret_cast<const float4*>(s_rescale)[r / 4];
             ref[r] = m.x; ref[r + 1] = m.y; ref[r + 2] = m.z; ref[r + 3] = m.w;
             scale[r] = x.x; scale[r + 1] = x.y; scale[r + 2] = x.z; scale[r + 3] = x.w;
           }
 #pragma unroll
-          for (int r = 0; r < R; ++r) acc[r] *= scale[r];
+          for (int r = 0; r < R; ++r) {
+            if (r % 4 == 0 && r >= p.rows) break;
+            acc[r] *= scale[r];
+          }
           if (i >= 2) {   // behind the group's last P.V
-            mbar_wait_rows(bars + L::kODone + group, ((J >> 1) - 1) & 1, ab, kPgODone);
+            paged_wait(bars + L::kODone + group, ((J >> 1) - 1) & 1, ab, kPgODone);
             tc_fence_after_sync();
 #pragma unroll
             for (int c = 0; c < R; c += 16) {
@@ -375,9 +384,10 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
           }
         }
         // the operand's buffer is free behind the group's last P.V
-        if (J >= 2) mbar_wait_rows(bars + L::kODone + group, ((J >> 1) - 1) & 1, ab, kPgODone);
+        if (J >= 2) paged_wait(bars + L::kODone + group, ((J >> 1) - 1) & 1, ab, kPgODone);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
+          if (r % 4 == 0 && r >= p.rows) break;   // four rows at a time, those that there are
           const float x = fast_exp2(s[r] - ref[r]);
           acc[r] += x;
           const uint32_t two = pack2<kBf16>(x, 0.0f);
@@ -395,7 +405,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
       sync();
       if (key0 < R) s_sum[key0] = (s_warp[key0] + s_warp[R + key0]) + (s_warp[2 * R + key0] + s_warp[3 * R + key0]);
       const int Jl = J0 + u.n - 1, mine = (Jl & 1) == group ? Jl : Jl - 1;   // the group's last tile
-      if (mine >= J0) mbar_wait_rows(bars + L::kODone + group, (mine >> 1) & 1, ab, kPgODone);
+      if (mine >= J0) paged_wait(bars + L::kODone + group, (mine >> 1) & 1, ab, kPgODone);
       if (named_sync_or(3, 256, *abort_flag != 0)) break;   // both groups; all warps together
       tc_fence_after_sync();
       const bool has0 = ((Jl & 1) == 0 ? Jl : Jl - 1) >= J0, has1 = ((Jl & 1) == 1 ? Jl : Jl - 1) >= J0;
@@ -456,7 +466,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
       PagedWalk u = make_walk(), ahead = make_walk();
       auto split = [&](int ui) -> bool {
         const int qb = ui & 1;
-        if (ui >= 2 && !warp_all(mbar_wait(bars + L::kQEmpty + qb, ((ui >> 1) - 1) & 1, ab, kPgQEmpty))) return false;
+        if (ui >= 2 && !warp_all(paged_wait(bars + L::kQEmpty + qb, ((ui >> 1) - 1) & 1, ab, kPgQEmpty))) return false;
         paged_split_queries<D, kBf16, L::kPieces, L::kConvWarps>(p, ahead, tab.row[ahead.b], ct, sQ + qb * L::kQBytes, R * D, reinterpret_cast<float*>(smem + L::kOffQs) + (ui & 3) * R);
         if (lane == 0) mbar_arrive(bars + L::kQFull + qb);
         return true;
@@ -468,13 +478,11 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
         if (ahead.next()) ok = split(ui + 1);
         for (int i = 0; i < u.n && ok; ++i, ++J) {
           const int sc = J % L::kScales, raw = J % L::kRaw, st = J % L::kStagesV;
-          ok = warp_all(mbar_wait(bars + L::kScFull + sc, (J / L::kScales) & 1, ab, kPgScales));
-          ok = ok && warp_all(mbar_wait(bars + L::kRawFull + raw, (J / L::kRaw) & 1, ab, kPgRawFull));
-          ok = ok && warp_all(mbar_wait(bars + L::kVEmpty + st, ((J / L::kStagesV) & 1) ^ 1, ab, kPgVEmpty));
+          ok = warp_all(paged_wait(bars + L::kScFull + sc, (J / L::kScales) & 1, ab, kPgScales));
+          ok = ok && warp_all(paged_wait(bars + L::kRawFull + raw, (J / L::kRaw) & 1, ab, kPgRawFull));
+          ok = ok && warp_all(paged_wait(bars + L::kVEmpty + st, ((J / L::kStagesV) & 1) ^ 1, ab, kPgVEmpty));
           if (!ok) break;
-          int a, e;
-          u.rows_of(i, a, e);
-          paged_widen<D, kBf16, L::kConvWarps>(smem + L::kOffRaw + raw * L::kRawBytes, smem + L::kOffScales + (sc * 2 + 1) * N, sV + st * L::kTileBytes, ct, a, e);
+          paged_widen<D, kBf16, L::kConvWarps>(smem + L::kOffRaw + raw * L::kRawBytes, smem + L::kOffScales + (sc * 2 + 1) * N, sV + st * L::kTileBytes, ct);
           if (lane == 0) {
             mbar_arrive(bars + L::kVFull + st);
             mbar_arrive(bars + L::kRawEmpty + raw);
