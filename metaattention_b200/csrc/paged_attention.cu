@@ -17,8 +17,10 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant_
   if (row >= p.rows) return;
   const int4 cut = __ldcg(p.cut + c_lo);
   if (cut.w < 0) return;
-  const int g = p.head_major ? row / p.per_tile : row % p.group, qi = p.head_major ? row % p.per_tile : row / p.group;
-  const int tok = cut.z * p.per_tile + qi, head = cut.y * p.group + g;
+  const int t = row / kPgTile, r = row - t * kPgTile;   // query tile and its row
+  const int g = p.head_major ? r / p.tile_pos : r % p.group, qi = p.head_major ? r % p.tile_pos : r / p.group;
+  if (r >= p.tile_pos * p.group) return;
+  const int tok = cut.z * p.per_tile + t * p.tile_pos + qi, head = cut.y * p.group + g;
   int row0 = 0, fresh = p.seq;
   if (p.cu != nullptr) {
     row0 = min(max(p.cu[cut.x], 0), p.seq);
@@ -98,9 +100,9 @@ inline int plan_paged(const AttnB200PagedAttnArgs* a, int sms, PagedPlan* d) {
   // A few rows a sequence: their own kernel.  How many a packed sequence has the host does not know; where they are less than
   // two on average a longer one among them costs a walk over its keys for each kPgFew of its rows.
   d->few = d->group <= kPgFew && (packed ? a->seq < 2LL * c.batch : static_cast<long long>(d->group) * a->seq <= kPgFew);
-  const int most_rows = d->few ? kPgFew : kPgTile;
-  d->per_tile = std::min(most_rows / d->group, a->seq);
-  d->rows = d->per_tile * d->group;
+  d->tile_pos = std::min((d->few ? kPgFew : kPgTile) / d->group, a->seq);
+  d->per_tile = d->few || a->seq <= d->tile_pos ? d->tile_pos : 2 * d->tile_pos;
+  d->rows = (d->per_tile > d->tile_pos ? kPgTile : 0) + d->tile_pos * d->group;
   const long long most_kv = static_cast<long long>(c.max_blocks) * c.page_size;
   if (most_kv > 0x3fffffff) return ATTN_B200_E_UNSUPPORTED;
   const long long q_tiles = packed ? a->seq / d->per_tile + c.batch : static_cast<long long>(c.batch) * ((a->seq + d->per_tile - 1) / d->per_tile);
@@ -155,14 +157,21 @@ int paged_setup(const AttnB200PagedAttnArgs* a, const PagedPlan& d, int* status,
   const bool packed = a->cu_seqlens != nullptr, codes = c.dtype == ATTN_B200_DTYPE_E4M3;
   const int D = c.head_dim, box = std::min(c.page_size, kPgTile);
   int rc;
-  if (codes) {   // keys are an operand as they come; values are widened first; queries are read and split into parts
+  if (codes && d.few) {   // queries are read and split into parts
     const bool aligned = (reinterpret_cast<uintptr_t>(a->q) & 15) == 0;
     const int extent[3] = {packed ? 1 : c.batch, a->seq, a->heads};
     for (int i = 0; i < 3; ++i) {
       if (!aligned || (extent[i] > 1 && a->q_stride[i] % 8 != 0)) return ATTN_B200_E_UNSUPPORTED;
       p.qs[i] = extent[i] > 1 ? a->q_stride[i] : 0;
     }
-    rc = encode_codes_map(&m->k, &p.ok, c.k, c, c.k_stride, box, D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+    rc = ATTN_B200_OK;
+  } else {
+    rc = encode_rows_map(&m->q, &p.oq, a->q, a->dtype, D, packed ? 1 : c.batch, a->seq, a->heads, a->q_stride, d.tile_pos, d.group);
+    p.head_major = p.oq.pos_s < p.oq.pos_h ? 1 : 0;
+  }
+  if (rc != ATTN_B200_OK) return rc;
+  if (codes) {   // keys are an operand as they come for a few rows; else they are widened first, as values are
+    rc = encode_codes_map(&m->k, &p.ok, c.k, c, c.k_stride, box, !d.few ? CU_TENSOR_MAP_SWIZZLE_NONE : D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
     if (rc == ATTN_B200_OK) rc = encode_codes_map(&m->v, &p.ov, c.v, c, c.v_stride, box, CU_TENSOR_MAP_SWIZZLE_NONE);
     const int pool[3] = {c.num_pages, c.page_size, c.heads_kv};
     for (int i = 0; i < 3; ++i) {
@@ -170,10 +179,8 @@ int paged_setup(const AttnB200PagedAttnArgs* a, const PagedPlan& d, int* status,
       p.scale_stride[1][i] = pool[i] > 1 ? c.v_scale_stride[i] : 0;
     }
   } else {
-    rc = encode_rows_map(&m->q, &p.oq, a->q, a->dtype, D, packed ? 1 : c.batch, a->seq, a->heads, a->q_stride, d.per_tile, d.group);
-    if (rc == ATTN_B200_OK) rc = encode_rows_map(&m->k, &p.ok, c.k, a->dtype, D, c.num_pages, c.page_size, c.heads_kv, c.k_stride, box);
+    rc = encode_rows_map(&m->k, &p.ok, c.k, a->dtype, D, c.num_pages, c.page_size, c.heads_kv, c.k_stride, box);
     if (rc == ATTN_B200_OK) rc = encode_rows_map(&m->v, &p.ov, c.v, a->dtype, D, c.num_pages, c.page_size, c.heads_kv, c.v_stride, box);
-    p.head_major = p.oq.pos_s < p.oq.pos_h ? 1 : 0;
   }
   if (rc != ATTN_B200_OK) return rc;
   p.q = static_cast<const uint16_t*>(a->q);
@@ -195,7 +202,7 @@ int paged_setup(const AttnB200PagedAttnArgs* a, const PagedPlan& d, int* status,
   p.seq = a->seq;
   p.per_tile = d.per_tile;
   p.rows = d.rows;
-  p.rows_pad = (d.rows + 7) / 8 * 8;
+  p.tile_pos = d.tile_pos;
   p.max_blocks = c.max_blocks;
   p.pages = c.num_pages;
   while ((1 << p.page_shift) < c.page_size) ++p.page_shift;

@@ -35,9 +35,9 @@ struct PagedParams {
   const int* table;
   long long table_stride;
   int batch, heads, heads_kv, group, seq;
-  int per_tile;                  // query positions of a tile
-  int rows, rows_pad;            // group * per_tile; padded to a multiple of 8
-  int q_bufs, q_bytes;            // paged_chunk.cu: query tiles in shared memory and the bytes of one
+  int per_tile;                  // query positions of a unit
+  int tile_pos;                  // and of one of its tiles of query rows (paged_chunk.cu has two)
+  int rows;                      // rows of a partial result: 128 to a tile, the last one's used ones
   int head_major;                // row = g * per_tile + i (1) or i * group + g (0): the order the tensor map delivers
   int max_blocks, page_shift, pages, box_shift;   // rows of a box: min(page, 128)
   int causal, window;
@@ -293,6 +293,13 @@ __device__ __forceinline__ uint2 widen4(uint32_t codes) {
   constexpr int kShift = kBf16 ? 4 : 1;
   return make_uint2((codes & 0x007f007fu) * (256u >> kShift) + (codes & 0x00800080u) * 256u, (codes & 0x80008000u) | ((codes & 0x7f007f00u) >> kShift));
 }
+// The same in order: for K, whose columns meet those of Q.
+template <bool kBf16>
+__device__ __forceinline__ uint2 widen4_ordered(uint32_t codes) {
+  constexpr int kShift = kBf16 ? 4 : 1;
+  const uint32_t lo = __byte_perm(codes, 0, 0x1404), hi = __byte_perm(codes, 0, 0x3424);
+  return make_uint2((lo & 0x80008000u) | ((lo & 0x7f007f00u) >> kShift), (hi & 0x80008000u) | ((hi & 0x7f007f00u) >> kShift));
+}
 // The column that a place of a widened row holds.
 __host__ __device__ constexpr int paged_column(int place) { return (place & ~3) | ((place & 1) << 1) | ((place >> 1) & 1); }
 template <bool kBf16>
@@ -430,7 +437,7 @@ __device__ __forceinline__ void paged_split_queries(const PagedParams& p, const 
 }
 
 // A tile of V from codes to 16 bits, by kWarps warps: chunks of 128-byte rows, swizzled as TMA would have written them.
-template <int D, bool kBf16, int kWarps>
+template <int D, bool kBf16, int kWarps, bool kOrdered = false>
 __device__ __forceinline__ void paged_widen(const uint8_t* src, const uint8_t* exponents, uint8_t* dst, int ct) {
   constexpr int kUnits = D / 16, kStep = 32 * kWarps / kUnits;   // pieces of 16 columns of a row, rows at a time
   const int unit = ct % kUnits;
@@ -464,7 +471,7 @@ __device__ __forceinline__ void paged_widen(const uint8_t* src, const uint8_t* e
     uint32_t w[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const uint2 x = widen4<kBf16>(c4[k]);
+      const uint2 x = kOrdered ? widen4_ordered<kBf16>(c4[k]) : widen4<kBf16>(c4[k]);
       w[2 * k] = x.x;
       w[2 * k + 1] = x.y;
     }
@@ -491,7 +498,7 @@ __device__ __forceinline__ void paged_widen(const uint8_t* src, const uint8_t* e
 }
 
 struct PagedPlan {
-  int group, per_tile, rows, ctas;
+  int group, per_tile, tile_pos, rows, ctas;
   bool few;          // paged_tokens.cu, else paged_chunk.cu
   long long off_lse, off_cut, bytes;
 };
