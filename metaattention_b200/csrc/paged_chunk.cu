@@ -2,13 +2,13 @@
 //
 // A unit is two tiles of 128 query rows of one KV head (half of the reads of K and V that one tile makes: at 128 rows to 64 KB of
 // keys and values the L2 cache is the bound); each KV tile meets both.
-//   warps 0-3, 4-7   softmax of a query tile each, one query row a thread: scores from tensor memory, P over them
-//   8, 9             loads of K and Q, of V
-//   10, 11           issue S = Q K^T, O += P V: with one warp for both its waits and bookkeeping stood in front of an idle pipe,
-//                    2130 cycles for a tile of 128 x 128 where the pipe needs 1024
-//   12, 13-19        8-bit caches: exponents of the rows; K and V in 16 bits (paged_common.cuh).  Beside them a softmax thread has no
-//                    room for a row of scores and reads them twice.
-// A tile's chain is scores -> softmax -> P.V -> its next scores (over P); the other tile's runs beside it.
+//   softmax          16-bit caches: two threads to a query row, eight warps to a query tile.  The scores leave their buffer for
+//                    registers as soon as they are there and P has columns of its own, so the next scores are computed under the
+//                    exponentials.  8-bit caches: four warps to a tile (the others widen), which have no room for a row and read
+//                    its scores twice, P over them; the tile's next scores wait for its P.V, the other tile's runs beside it.
+//   four warps       loads of K and Q, of V; issue S = Q K^T, O += P V: with one warp for both its waits and bookkeeping stood in
+//                    front of an idle pipe, 2130 cycles for a tile of 128 x 128 where the pipe needs 1024
+//   eight more       8-bit caches: exponents of the rows; K and V in 16 bits (paged_common.cuh)
 #include <cstring>
 
 #include "paged_common.cuh"
@@ -18,7 +18,10 @@ namespace b200 {
 template <int D, bool k8Bit>
 struct ChunkSmem {
   static constexpr int kConvWarps = 7;                               // with them twenty warps: 96 registers a thread
-  static constexpr int kThreads = 384 + (k8Bit ? 32 + 32 * kConvWarps : 0);
+  static constexpr int kRowThreads = k8Bit ? 1 : 2;                  // threads of a query row
+  static constexpr int kSoftmaxWarps = 8 * kRowThreads;
+  static constexpr int kThreads = (kSoftmaxWarps + 4) * 32 + (k8Bit ? 32 + 32 * kConvWarps : 0);
+  static constexpr int kScores = k8Bit || D == 64 ? 2 : 1;           // score buffers: one for each query tile, or one in turn
   static constexpr int kTileBytes = kPgTile * D * 2, kRawBytes = kPgTile * D;
   static constexpr int kStagesK = D == 128 ? 2 : 4, kStagesV = D == 128 ? (k8Bit ? 1 : 2) : 4;
   static constexpr int kRawK = k8Bit ? (D == 128 ? 2 : 3) : 0, kRawV = k8Bit ? (D == 128 ? 1 : 2) : 0;   // tiles of codes
@@ -33,9 +36,10 @@ struct ChunkSmem {
   static constexpr int kQFull = 0, kQEmpty = 1, kSFull = 2, kPReady = 4, kODone = 6, kOFree = 8, kKFull = 10, kKEmpty = kKFull + kStagesK;
   static constexpr int kVFull = kKEmpty + kStagesK, kVEmpty = kVFull + kStagesV, kRawKFull = kVEmpty + kStagesV, kRawKEmpty = kRawKFull + kRawK;
   static constexpr int kRawVFull = kRawKEmpty + kRawK, kRawVEmpty = kRawVFull + kRawV, kScFull = kRawVEmpty + kRawV, kScEmpty = kScFull + kScales;
-  static constexpr int kNumBars = kScEmpty + kScales;
+  static constexpr int kSFree = kScEmpty + kScales, kNumBars = kSFree + 2;   // the scores of a buffer are in registers
   static constexpr int kOffMisc = kOffBar + 8 * kNumBars;
-  static constexpr int kOffTables = kOffMisc + 16;
+  static constexpr int kOffExchange = kOffMisc + 16;                 // float [2][2][2][128]: by step, tile and half, the row's
+  static constexpr int kOffTables = kOffExchange + (k8Bit ? 0 : 8 * kPgTile * 4);
   static constexpr int kBytes = kOffTables + PagedTables::kBytes;    // the dynamic shared memory is declared 1024-byte aligned
   static_assert(kBytes <= 232448, "shared memory layout exceeds an SM");
 };
@@ -46,7 +50,10 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
   using L = ChunkSmem<D, k8Bit>;
   using F = SoftmaxFunctor;
   constexpr int N = kPgTile, KC = D / 64, kChunk = N * 128;
-  constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;
+  constexpr int kKWarp = L::kSoftmaxWarps, kVWarp = kKWarp + 1, kQkWarp = kKWarp + 2, kPvWarp = kKWarp + 3;
+  // accumulators; P, or P over the scores; scores
+  constexpr uint32_t kTmemCols = 512, kColO = 0, kColS = 512 - L::kScores * N, kColP = k8Bit ? kColS : 2 * D, kPStep = k8Bit ? N : N / 2;
+  static_assert(kColP + (k8Bit ? 0 : N) <= kColS && 2 * D <= kColS, "tensor memory layout");
 
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem + L::kOffQ;
@@ -65,14 +72,14 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
   static_assert(L::kBytes + 65536 > 233472, "a CTA with tensor memory could share the SM");
   pdl_launch_dependents();
 
-  if (warp == 10) {
+  if (warp == kQkWarp) {
     for (int i = lane; i < L::kNumBars; i += 32) {
       int count = 1;
-      if ((i >= L::kPReady && i < L::kODone) || (i >= L::kOFree && i < L::kKFull)) count = 4;
+      if ((i >= L::kPReady && i < L::kODone) || (i >= L::kOFree && i < L::kKFull) || i >= L::kSFree) count = 4 * L::kRowThreads;
       if constexpr (k8Bit) {   // written, or read, by the warps that widen
         if ((i >= L::kKFull && i < L::kKEmpty) || (i >= L::kVFull && i < L::kVEmpty) || (i >= L::kRawKEmpty && i < L::kRawVFull) || (i >= L::kRawVEmpty && i < L::kScFull))
           count = L::kConvWarps;
-        if (i >= L::kScFull) count = i < L::kScEmpty ? 32 : L::kConvWarps;
+        if (i >= L::kScFull && i < L::kSFree) count = i < L::kScEmpty ? 32 : L::kConvWarps;
       }
       mbar_init(bars + i, count);
     }
@@ -84,7 +91,7 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
       tma_prefetch_desc(&maps.v);
     }
   }
-  if (warp == 11) {
+  if (warp == kPvWarp) {
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
@@ -105,23 +112,16 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
   const PagedShare share(p, tab);
   const bool run_cta = warp_all(share.t1 > share.t0 && !*abort_flag);
   auto make_walk = [&]() { return PagedWalk(p, tab.cum, tab.len, tab.row, share.t0, share.t1); };
-  // whether any row of the unit's query tile t sees a key of its i-th KV tile
-  struct Sees {
-    int begin[2], end[2];
-    __device__ Sees(const PagedParams& p, const PagedWalk& u) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int tok = u.qt * p.per_tile + t * p.tile_pos, n = min(p.tile_pos, u.fresh - tok);   // the tile's tokens
-        const int first = u.len - u.fresh + tok, last = first + n - 1;
-        end[t] = n <= 0 || (t == 1 && p.per_tile <= p.tile_pos) ? 0 : p.causal ? min(u.len, last + 1) : u.len;
-        begin[t] = p.window > 0 ? max(0, first - p.window + 1) : 0;
-      }
-    }
-    __device__ bool operator()(int t, int kv0) const { return kv0 < (t == 0 ? end[0] : end[1]) && kv0 + kPgTile > (t == 0 ? begin[0] : begin[1]); }
+  // keys [begin, end) that any row of the unit's query tile t sees
+  auto keys_of = [&](const PagedWalk& u, int t, int& begin, int& end) {
+    const int tok = u.qt * p.per_tile + t * p.tile_pos, n = min(p.tile_pos, u.fresh - tok);   // the tile's tokens
+    const int first = u.len - u.fresh + tok, last = first + n - 1;
+    end = n <= 0 || (t == 1 && p.per_tile <= p.tile_pos) ? 0 : p.causal ? min(u.len, last + 1) : u.len;
+    begin = p.window > 0 ? max(0, first - p.window + 1) : 0;
   };
 
   if (!run_cta) {
-  } else if (warp == 8) {
+  } else if (warp == kKWarp) {
     // ======================= loads of keys and queries =======================
     paged_load<k8Bit ? 1 : KC, k8Bit ? D : 128, k8Bit ? L::kRawK : L::kStagesK>(
         p, make_walk(), &maps.k, p.ok, k8Bit ? smem + L::kOffRawK : sK, k8Bit ? L::kRawBytes : L::kTileBytes, kChunk, bars + (k8Bit ? L::kRawKFull : L::kKFull),
@@ -137,23 +137,25 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
           }
           return true;
         });
-  } else if (warp == 9) {
+  } else if (warp == kVWarp) {
     // ======================= loads of values =======================
     paged_load<k8Bit ? 1 : KC, k8Bit ? D : 128, k8Bit ? L::kRawV : L::kStagesV>(
         p, make_walk(), &maps.v, p.ov, k8Bit ? smem + L::kOffRawV : sV, k8Bit ? L::kRawBytes : L::kTileBytes, kChunk, bars + (k8Bit ? L::kRawVFull : L::kVFull),
         bars + (k8Bit ? L::kRawVEmpty : L::kVEmpty), ab, kPgVEmpty, [](const PagedWalk&, int) { return true; });
-  } else if (warp == 10 || warp == 11) {
+  } else if (warp == kQkWarp || warp == kPvWarp) {
     // ======================= issue S = Q K^T and O += P V (converged, one elected lane a batch) =======================
     auto wait = [&](uint64_t* bar, uint32_t parity, int site) -> bool { return warp_all(paged_wait(bar, parity, ab, site)); };
     PagedWalk u = make_walk();
     bool ok = true;
-    int st = 0, own[2] = {0, 0};   // scores, or products, so far of each query tile
+    int st = 0, own[2] = {0, 0}, all = 0;   // scores, or products, so far of each query tile, and of both
     uint32_t par = 0;
-    if (warp == 10) {
+    if (warp == kQkWarp) {
       constexpr uint32_t idesc = make_idesc_f16(128, N, kBf16, false, false);
       const uint64_t q_desc0 = make_smem_desc(smem_u32(sQ), 16, 1024), k_desc0 = make_smem_desc(smem_u32(sK), 16, 1024);
       for (int ui = 0; ok && u.next(); ++ui) {
-        const Sees sees(p, u);
+        int begin[2], end[2];
+        keys_of(u, 0, begin[0], end[0]);
+        keys_of(u, 1, begin[1], end[1]);
         ok = wait(bars + L::kQFull, ui & 1, kPgQFull);
         for (int i = 0; i < u.n && ok; ++i) {
           const int kv0 = (u.lo + u.t0 + i) * N;
@@ -161,18 +163,24 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
           const uint64_t bk = k_desc0 + static_cast<uint64_t>(st * (L::kTileBytes >> 4));
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (!ok || !sees(t, kv0)) continue;
-            if (own[t] > 0) ok = wait(bars + L::kODone + t, (own[t] - 1) & 1, kPgODone);   // P of the last tile has been read
+            if (!ok || kv0 >= end[t] || kv0 + N <= begin[t]) continue;
+            const int buf = L::kScores == 2 ? t : 0, use = L::kScores == 2 ? own[t] : all;
+            if (k8Bit) {
+              if (own[t] > 0) ok = wait(bars + L::kODone + t, (own[t] - 1) & 1, kPgODone);   // the P in these columns has been read
+            } else if (use > 0) {
+              ok = wait(bars + L::kSFree + buf, (use - 1) & 1, kPgSFree);
+            }
             if (!ok) continue;
             tc_fence_after_sync();
             const uint64_t a = q_desc0 + static_cast<uint64_t>(t * (L::kTileBytes >> 4));
             if (elect_one()) {
 #pragma unroll
               for (int ch = 0; ch < KC; ++ch)
-                umma_ss_x4<2, 2>(tmem_base + kColS + t * N, a + ch * (kChunk >> 4), bk + ch * (kChunk >> 4), idesc, ch > 0 ? 1u : 0u);
+                umma_ss_x4<2, 2>(tmem_base + kColS + buf * N, a + ch * (kChunk >> 4), bk + ch * (kChunk >> 4), idesc, ch > 0 ? 1u : 0u);
               umma_commit(bars + L::kSFull + t);
             }
             ++own[t];
+            ++all;
           }
           if (ok && elect_one()) {   // behind the tile's scores, if any
             umma_commit(bars + L::kKEmpty + st);
@@ -189,7 +197,9 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
       constexpr uint32_t idesc = make_idesc_f16(128, D, kBf16, false, true);
       const uint64_t v_desc0 = make_smem_desc(smem_u32(sV), kChunk, 1024);
       for (int ui = 0; ok && u.next(); ++ui) {
-        const Sees sees(p, u);
+        int begin[2], end[2];
+        keys_of(u, 0, begin[0], end[0]);
+        keys_of(u, 1, begin[1], end[1]);
         bool begun[2] = {false, false};
         for (int i = 0; i < u.n && ok; ++i) {
           const int kv0 = (u.lo + u.t0 + i) * N;
@@ -201,7 +211,7 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
           const uint64_t bv = v_desc0 + static_cast<uint64_t>(st * (L::kTileBytes >> 4));
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (!ok || !sees(t, kv0)) continue;
+            if (!ok || kv0 >= end[t] || kv0 + N <= begin[t]) continue;
             if (!begun[t] && ui > 0) ok = wait(bars + L::kOFree + t, (ui - 1) & 1, kPgOFree);   // the last unit's rows have been read
             ok = ok && wait(bars + L::kPReady + t, own[t] & 1, kPgPReady);
             if (!ok) continue;
@@ -209,7 +219,7 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
             if (elect_one()) {
 #pragma unroll
               for (int g = 0; g < N / 64; ++g)
-                umma_ts_x4<8, 128>(tmem_base + kColO + t * D, tmem_base + kColS + t * N + g * 32, bv + g * 512, idesc, (begun[t] || g > 0) ? 1u : 0u);
+                umma_ts_x4<8, 128>(tmem_base + kColO + t * D, tmem_base + kColP + t * kPStep + g * 32, bv + g * 512, idesc, (begun[t] || g > 0) ? 1u : 0u);
               umma_commit(bars + L::kODone + t);
             }
             begun[t] = true;
@@ -224,13 +234,24 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
         }
       }
     }
-  } else if (warp < 8) {
-    // ======================= softmax: a query tile for four warps, a row a thread =======================
-    const int t = warp >> 2;
+  } else if (warp < L::kSoftmaxWarps) {
+    // ======================= softmax =======================
+    constexpr int RT = L::kRowThreads, TC = N / RT, OC = D / RT;   // threads of a row; columns of a thread, of scores and of o
+    const int t = warp / (4 * RT), half = RT == 1 ? 0 : (warp >> 2) & 1;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem_base + lane_base + kColS + t * N;
-    const uint32_t tO = tmem_base + lane_base + kColO + t * D;
+    const uint32_t tS = tmem_base + lane_base + kColS + (L::kScores == 2 ? t * N : 0) + half * TC;
+    const uint32_t tP = tmem_base + lane_base + kColP + t * kPStep + half * (TC / 2);
+    const uint32_t tO = tmem_base + lane_base + kColO + t * D + half * OC;
+    const int pair_bar = 1 + t * 4 + (warp & 3);   // of the two warps that share rows
+    float* xch = reinterpret_cast<float*>(smem + L::kOffExchange) + t * 2 * N + row;
+    int exchanges = 0;   // two buffers in turn: the partner may still read the last one's
+    auto exchange = [&](float mine) -> float {
+      float* x = xch + (exchanges++ & 1) * (4 * N);
+      x[half * N] = mine;
+      named_sync(pair_bar, 64);
+      return x[(half ^ 1) * N];
+    };
     const FunctorArgs fa{{p.scale}};
     const RowCtx ctx{0, 0, 0, 0, p.seq, 0, &fa};   // softmax asks for the scale only
     const int g = p.head_major ? row / p.tile_pos : row % p.group;
@@ -239,7 +260,8 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
     PagedWalk u = make_walk();
     int own = 0;   // tiles so far
     for (int ui = 0; u.next(); ++ui) {
-      const Sees sees(p, u);
+      int begin, end;
+      keys_of(u, t, begin, end);
       const int tok = u.qt * p.per_tile + t * p.tile_pos + qi;   // the row's new token
       const bool live = row < p.tile_pos * p.group && tok < u.fresh && t * p.tile_pos < p.per_tile;
       const bool any_live = __any_sync(0xffffffffu, live);
@@ -250,14 +272,20 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
       float rs[2];
       F::init(rs, ctx);
       bool begun = false;
-      for (int i = 0; i < u.n; ++i) {
-        const int kv0 = (u.lo + u.t0 + i) * N;
-        if (!sees(t, kv0)) continue;
+#pragma unroll 1
+      for (int kv0 = (u.lo + u.t0) * N, kv1 = kv0 + u.n * N; kv0 < kv1; kv0 += N) {
+        if (kv0 >= end || kv0 + N <= begin) continue;
         paged_wait(bars + L::kSFull + t, own & 1, ab, kPgSFull);
         ++own;
         if (!any_live) {   // nothing of this warp's rows is kept
+          // (its arrivals keep in step: one for the next P before the last P.V would count for that)
+          if (!k8Bit && begun) paged_wait(bars + L::kODone + t, own & 1, ab, kPgODone);
           begun = true;
-          if (lane == 0) mbar_arrive(bars + L::kPReady + t);
+          __syncwarp();
+          if (lane == 0) {
+            if (!k8Bit) mbar_arrive(bars + L::kSFree + (L::kScores == 2 ? t : 0));
+            mbar_arrive(bars + L::kPReady + t);
+          }
           continue;
         }
         tc_fence_after_sync();
@@ -265,21 +293,27 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
         const bool edge = __any_sync(0xffffffffu, e < N || a > 0);
         float o_scale = 1.0f;
         if constexpr (!k8Bit) {
-          float s[N];
+          float s[TC];
 #pragma unroll
-          for (int c = 0; c < N / 32; ++c) tmem_ld32f(tS + c * 32, &s[c * 32]);
+          for (int c = 0; c < TC / 32; ++c) tmem_ld32f(tS + c * 32, &s[c * 32]);
           tmem_wait_ld();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars + L::kSFree + (L::kScores == 2 ? t : 0));
           if (edge) {
+            const int e1 = e - half * TC, a1 = a - half * TC;
 #pragma unroll
-            for (int k = 0; k < N; ++k) s[k] = k < e && k >= a ? s[k] : -INFINITY;
+            for (int k = 0; k < TC; ++k) s[k] = k < e1 && k >= a1 ? s[k] : -INFINITY;
           }
-          o_scale = F::template tile_pieces<N, 4, false>(s, rs, ctx, [](float mx) { return mx; }, [&](int c) {
-            constexpr int W = N / 4 / 2;
-            uint32_t pk[W];
+          o_scale = F::template tile_pieces<TC, TC / 32>(s, rs, ctx, [&](float mx) { return fmaxf(mx, exchange(mx)); }, [&](int c) {
+            if (c == 0 && begun) {   // P's columns are free, and the accumulator is, behind the tile's last P.V
+              mbar_wait_rows(bars + L::kODone + t, own & 1, ab, kPgODone);   // (in line: a call would cost the row's registers)
+              tc_fence_after_sync();
+            }
+            uint32_t pk[16];
 #pragma unroll
-            for (int k = 0; k < W; ++k) pk[k] = pack2<kBf16>(s[c * 2 * W + 2 * k], s[c * 2 * W + 2 * k + 1]);
-            static_assert(W == 16, "a quarter of the row per store");
-            tmem_st16(tS + c * W, pk);
+            for (int k = 0; k < 16; ++k) pk[k] = pack2<kBf16>(s[c * 32 + 2 * k], s[c * 32 + 2 * k + 1]);
+            tmem_st16(tP + c * 16, pk);
           });
         } else {
           // twice, 32 columns at a time: for the maximum, then for P, over what has been read
@@ -326,13 +360,13 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
               add_x2(a0, a1, s[2 * k], s[2 * k + 1]);
               pk[k] = pack2<kBf16>(s[2 * k], s[2 * k + 1]);
             }
-            tmem_st16(tS + c / 2, pk);
+            tmem_st16(tP + c / 2, pk);
           }
           rs[1] += a0 + a1;
         }
-        if (begun && __any_sync(0xffffffffu, o_scale != 1.0f)) {   // (these scores were issued behind the last P.V)
+        if (begun && __any_sync(0xffffffffu, o_scale != 1.0f)) {   // (8 bits: these scores were issued behind the last P.V)
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
+          for (int c = 0; c < OC / 32; ++c) {
             float o[32];
             tmem_ld32f(tO + c * 32, o);
             tmem_wait_ld();
@@ -349,7 +383,12 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
       }
       // ---- end of a unit ----
       if (begun) paged_wait(bars + L::kODone + t, (own - 1) & 1, ab, kPgODone);
-      if (!warp_all(!*abort_flag)) break;
+      if constexpr (RT == 2) {
+        rs[1] += exchange(rs[1]);
+        if (!named_sync_and(pair_bar, 64, !*abort_flag)) break;
+      } else {
+        if (!warp_all(!*abort_flag)) break;
+      }
       tc_fence_after_sync();
       const float sum = rs[1], inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // no key: 0, and -inf
       const float lse = sum == 0.0f ? -INFINITY : logf(sum) + rs[0] * p.scale;
@@ -358,15 +397,13 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
       // a partial result: the unit's first share leaves it in the second slot of its CTA, the later ones in the first
       const long long slot = (2LL * cta + (u.t0 == 0 ? 1 : 0)) * p.rows + t * N + row;
       const long long at = p.cu != nullptr ? tab.row[u.b] + tok : tok;   // row of o
-      uint16_t* orow = static_cast<uint16_t*>(p.o) + (p.cu != nullptr ? 0 : u.b * p.o_sb) + at * p.o_ss + head * p.o_sh;
+      uint16_t* orow = static_cast<uint16_t*>(p.o) + (p.cu != nullptr ? 0 : u.b * p.o_sb) + at * p.o_ss + head * p.o_sh + half * OC;
       if (any_live) {
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = 0; c < OC / 32; ++c) {
           float o[32];
-          if (begun) {
-            tmem_ld32f(tO + c * 32, o);
-            tmem_wait_ld();
-          }
+          tmem_ld32f(tO + c * 32, o);
+          tmem_wait_ld();
 #pragma unroll
           for (int k = 0; k < 32; ++k) o[k] = begun ? o[k] * inv : 0.0f;
           if constexpr (k8Bit) {   // columns in their order
@@ -389,13 +426,13 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
                 reinterpret_cast<uint4*>(orow + c * 32)[v] = pk;
               }
             } else {
-              float4* dst = reinterpret_cast<float4*>(p.part_o + slot * D + c * 32);
+              float4* dst = reinterpret_cast<float4*>(p.part_o + slot * D + half * OC + c * 32);
 #pragma unroll
               for (int v = 0; v < 8; ++v) dst[v] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
             }
           }
         }
-        if (live) {
+        if (live && half == 0) {
           if (!whole) p.part_lse[slot] = lse;
           else if (p.lse != nullptr) p.lse[(p.cu != nullptr ? static_cast<long long>(head) : static_cast<long long>(u.b) * p.heads + head) * p.seq + at] = lse;
         }
@@ -449,7 +486,7 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
     for (int i = 0; i < 200; ++i) __nanosleep(1000);
     __syncthreads();
   }
-  if (warp == 11) {
+  if (warp == kPvWarp) {
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, kTmemCols);
   }

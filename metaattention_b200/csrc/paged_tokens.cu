@@ -294,7 +294,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
         if (lane == 0) mbar_arrive(bars + L::kSFree + sb);
         if constexpr (k8Bit) {
           const int slot = J % L::kScales;
-          paged_wait(bars + L::kScFull + slot, (J / L::kScales) & 1, ab, kPgScales);
+          mbar_wait_rows(bars + L::kScFull + slot, (J / L::kScales) & 1, ab, kPgScales);
           const float f = key_factor(smem[L::kOffScales + slot * 2 * N + key0]) * c2;
           const float4* qs = reinterpret_cast<const float4*>(smem + L::kOffQs) + (ui & 3) * (R / 4);
 #pragma unroll
@@ -369,7 +369,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
             acc[r] *= scale[r];
           }
           if (i >= 2) {   // behind the group's last P.V
-            paged_wait(bars + L::kODone + group, ((J >> 1) - 1) & 1, ab, kPgODone);
+            mbar_wait_rows(bars + L::kODone + group, ((J >> 1) - 1) & 1, ab, kPgODone);
             tc_fence_after_sync();
 #pragma unroll
             for (int c = 0; c < R; c += 16) {
@@ -384,7 +384,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
           }
         }
         // the operand's buffer is free behind the group's last P.V
-        if (J >= 2) paged_wait(bars + L::kODone + group, ((J >> 1) - 1) & 1, ab, kPgODone);
+        if (J >= 2) mbar_wait_rows(bars + L::kODone + group, ((J >> 1) - 1) & 1, ab, kPgODone);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           if (r % 4 == 0 && r >= p.rows) break;   // four rows at a time, those that there are

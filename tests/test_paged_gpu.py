@@ -309,6 +309,21 @@ def test_packed_mixture_leaves_padding_alone(codes, window):
 
 
 @pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("D,window", [(64, None), (64, 700), (128, None)])
+def test_long_packed_mixtures(codes, D, window):
+    """Single tokens on long contexts in units of many rows, most of which are nobody's: warps without a row keep in step with the
+    others of their tile.  Several calls, which agree to the bit."""
+    news = [40, 1, 1, 5, 1, 33, 1, 1]
+    lens = [1500, 1900, 700, 1200, 2300, 900, 1601, 130]
+    c, q, o, lse = run_attention(lens, news, 8, 2, D, 16, torch.float16, codes, packed=True, seed=9, window=window)
+    cu = torch.tensor([sum(news[:i]) for i in range(len(news) + 1)], dtype=torch.int32).cuda()
+    for _ in range(20):
+        again, lse2 = c.cache.attention(q.cuda(), c.block_table, c.cache_seqlens, cu_seqlens=cu, window=window, return_lse=True)
+        assert torch.equal(again, o) and torch.equal(lse2, lse)
+    assert lib.last_device_status() == 0
+
+
+@pytest.mark.parametrize("codes", [False, True])
 @pytest.mark.parametrize("group", [1, 3, 5, 7, 16, 33, 64, 128])
 def test_group_sizes(codes, group):
     run_attention([40, 150], [9, 9], group, 1, 64, 16, torch.bfloat16, codes, seed=group)
