@@ -43,10 +43,9 @@ struct AppendParams {
   AttnB200Rotary rot;
 };
 
-// 16 values of a head as floats: columns c0 .. c0 + 7 and c1 .. c1 + 7
+// 16 values of a head as floats
 template <bool kBf16>
-__device__ __forceinline__ void load16(const uint16_t* row, int c0, int c1, float (&x)[16]) {
-  const uint4 lo = *reinterpret_cast<const uint4*>(row + c0), hi = *reinterpret_cast<const uint4*>(row + c1);
+__device__ __forceinline__ void unpack16(const uint4 lo, const uint4 hi, float (&x)[16]) {
   const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -64,8 +63,10 @@ __device__ __forceinline__ uint32_t codes4(const float* x) {
 
 // A thread owns 16 columns of a token and walks its heads, so that a k's angles are made once; the D / 16 threads of a row
 // are neighbours in a warp, for the row's largest magnitude.
+constexpr int kAppendThreads = 128;
+
 template <int D, bool kBf16, bool k8Bit>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendParams p) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int kUnits = D / 16;
@@ -76,84 +77,91 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p)
   const int lane = static_cast<int>(group - row * p.lanes);
   bool live = row < p.rows;
   int b = 0, t = static_cast<int>(row), pos = -1;
+  if (live && p.cu == nullptr) {
+    b = t / p.seq;
+    t -= b * p.seq;
+  }
+  // columns of k: two pieces of 8 whose pairs this thread turns; v: 16 in a row
+  int c0 = unit * 16, c1 = c0 + 8;
+  const bool mine = unit < p.rot.dim / 16;   // its columns of k turn
+  if (mine && !p.rot.interleaved) {
+    c0 = unit * 8;
+    c1 = c0 + p.rot.dim / 2;
+  }
+  const long long in_b = p.cu == nullptr ? b : 0;
+  uint4 lo[2], hi[2];
+  auto load = [&](int h, uint4 (&lo)[2], uint4 (&hi)[2]) {
+    if (live && h < p.c.heads) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const uint16_t* src = p.in[w] + in_b * p.is[w][0] + t * p.is[w][1] + h * p.is[w][2];
+        lo[w] = *reinterpret_cast<const uint4*>(src + (w == 0 ? c0 : unit * 16));
+        hi[w] = *reinterpret_cast<const uint4*>(src + (w == 0 ? c1 : unit * 16 + 8));
+      }
+    }
+  };
+  lo[0] = lo[1] = hi[0] = hi[1] = make_uint4(0, 0, 0, 0);
+  load(lane, lo, hi);   // on its way while the row's place and angles are found
   if (live) {
     if (p.cu == nullptr) {
-      b = t / p.seq;
-      t -= b * p.seq;
       pos = p.c.lens[b] - p.seq + t;
     } else {
-      int lo = 0, hi = p.c.batch;   // the last sequence that begins at or before the row
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (p.cu[mid] <= t) lo = mid; else hi = mid;
+      int first = 0, behind = p.c.batch;   // the last sequence that begins at or before the row
+      while (behind - first > 1) {
+        const int mid = (first + behind) >> 1;
+        if (p.cu[mid] <= t) first = mid; else behind = mid;
       }
-      b = lo;
+      b = first;
       const int end = p.cu[b + 1];
       live = t >= p.cu[b] && t < end;
       pos = p.c.lens[b] - (end - t);
-      }
+    }
   }
   live = live && pos >= 0;
   const int page = live ? page_of(p.c, b, pos) : -1;
   live = live && page >= 0;
   // the threads of a row agree, and rows that have no place stay for the shuffles
   const int in_page = pos & ((1 << p.c.page_shift) - 1);
-  const bool turns = p.rot.dim > 0;
-  // columns of k: two pieces of 8 whose pairs this thread turns; v: 16 in a row
-  int c0 = unit * 16, c1 = c0 + 8;
-  bool mine = false;
   float2 cs[8];
-  if (turns && live) {
-    const int pairs = p.rot.dim / 16;   // threads whose columns turn
-    mine = unit < pairs;
-    if (mine) {
-      if (!p.rot.interleaved) {
-        c0 = unit * 8;
-        c1 = c0 + p.rot.dim / 2;
-      }
+  if (mine && live) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) cs[i] = rotary_cos_sin<false>(p.rot.turns[unit * 8 + i], pos, p.rot.magnitude, false);
-    }
+    for (int i = 0; i < 8; ++i) cs[i] = rotary_cos_sin<false>(p.rot.turns[unit * 8 + i], pos, p.rot.magnitude, false);
   }
-  const long long in_b = p.cu == nullptr ? b : 0;
+#pragma unroll 1
   for (int h0 = 0; h0 < p.c.heads; h0 += p.lanes) {
     const int h = h0 + lane;
     const bool on = live && h < p.c.heads;
+    uint4 lo_next[2], hi_next[2];
+    load(h + p.lanes, lo_next, hi_next);
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const int a0 = w == 0 ? c0 : unit * 16, a1 = w == 0 ? c1 : unit * 16 + 8;
-      const uint16_t* src = p.in[w] + in_b * p.is[w][0] + t * p.is[w][1] + h * p.is[w][2];
       uint8_t* dst = p.c.kv[w] + (page * p.c.stride[w][0] + in_page * p.c.stride[w][1] + h * p.c.stride[w][2]) * (k8Bit ? 1 : 2);
-      if (!k8Bit && (w == 1 || !mine)) {
+      const bool turned = w == 0 && mine;
+      if (!k8Bit && !turned) {
         if (on) {
-          const uint4 lo = *reinterpret_cast<const uint4*>(src + a0), hi = *reinterpret_cast<const uint4*>(src + a1);
-          *reinterpret_cast<uint4*>(dst + 2 * a0) = lo;
-          *reinterpret_cast<uint4*>(dst + 2 * a1) = hi;
+          *reinterpret_cast<uint4*>(dst + 2 * a0) = lo[w];
+          *reinterpret_cast<uint4*>(dst + 2 * a1) = hi[w];
         }
+        lo[w] = lo_next[w];
+        hi[w] = hi_next[w];
         continue;
       }
       float x[16];
+      unpack16<kBf16>(lo[w], hi[w], x);
+      if (turned) {
+        if (p.rot.interleaved) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = 0.0f;
-      if (on) {
-        load16<kBf16>(src, a0, a1, x);
-        if (w == 0 && mine) {
-          if (p.rot.interleaved) {
+          for (int i = 0; i < 8; ++i) rotary_turn(x[2 * i], x[2 * i + 1], cs[i]);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) rotary_turn(x[2 * i], x[2 * i + 1], cs[i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) rotary_turn(x[i], x[8 + i], cs[i]);
-          }
+          for (int i = 0; i < 8; ++i) rotary_turn(x[i], x[8 + i], cs[i]);
         }
       }
       if constexpr (!k8Bit) {
         if (on) {
-          uint4 lo, hi;
-          lo.x = pack2<kBf16>(x[0], x[1]); lo.y = pack2<kBf16>(x[2], x[3]); lo.z = pack2<kBf16>(x[4], x[5]); lo.w = pack2<kBf16>(x[6], x[7]);
-          hi.x = pack2<kBf16>(x[8], x[9]); hi.y = pack2<kBf16>(x[10], x[11]); hi.z = pack2<kBf16>(x[12], x[13]); hi.w = pack2<kBf16>(x[14], x[15]);
-          *reinterpret_cast<uint4*>(dst + 2 * a0) = lo;
-          *reinterpret_cast<uint4*>(dst + 2 * a1) = hi;
+          *reinterpret_cast<uint4*>(dst + 2 * a0) = make_uint4(pack2<kBf16>(x[0], x[1]), pack2<kBf16>(x[2], x[3]), pack2<kBf16>(x[4], x[5]), pack2<kBf16>(x[6], x[7]));
+          *reinterpret_cast<uint4*>(dst + 2 * a1) = make_uint4(pack2<kBf16>(x[8], x[9]), pack2<kBf16>(x[10], x[11]), pack2<kBf16>(x[12], x[13]), pack2<kBf16>(x[14], x[15]));
         }
       } else {
         // the largest magnitude as the bits of a float, which order like the magnitudes do; NaN and infinities on top
@@ -169,13 +177,14 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p)
         if (on) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] = finite ? x[i] * inv : __uint_as_float(0x7fffffffu);
-          const uint2 lo = make_uint2(codes4(x), codes4(x + 4)), hi = make_uint2(codes4(x + 8), codes4(x + 12));
-          *reinterpret_cast<uint2*>(dst + a0) = lo;
-          *reinterpret_cast<uint2*>(dst + a1) = hi;
+          *reinterpret_cast<uint2*>(dst + a0) = make_uint2(codes4(x), codes4(x + 4));
+          *reinterpret_cast<uint2*>(dst + a1) = make_uint2(codes4(x + 8), codes4(x + 12));
           if (unit == 0)
             p.c.scale[w][page * p.c.scale_stride[w][0] + in_page * p.c.scale_stride[w][1] + h * p.c.scale_stride[w][2]] = static_cast<uint8_t>(byte);
         }
       }
+      lo[w] = lo_next[w];
+      hi[w] = hi_next[w];
     }
   }
 }
@@ -210,10 +219,20 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const ReadParams p) {
   pdl_wait();
   constexpr int kUnits = D / 16;
   for (long long id = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; id < p.items; id += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const int unit = static_cast<int>(id % kUnits);
-    const long long row = id / kUnits, token = row / p.c.heads;   // (sequence, position)
-    const int h = static_cast<int>(row - token * p.c.heads);
-    const int b = static_cast<int>(token / p.max_len), t = static_cast<int>(token - static_cast<long long>(b) * p.max_len);
+    int unit, h, b, t;
+    if (p.items <= 0x7fffffff) {   // 64-bit divisions cost ten times as much
+      const int i = static_cast<int>(id), row = i / kUnits, token = row / p.c.heads;
+      unit = i - row * kUnits;
+      h = row - token * p.c.heads;
+      b = token / p.max_len;
+      t = token - b * p.max_len;
+    } else {
+      const long long row = id / kUnits, token = row / p.c.heads;
+      unit = static_cast<int>(id - row * kUnits);
+      h = static_cast<int>(row - token * p.c.heads);
+      b = static_cast<int>(token / p.max_len);
+      t = static_cast<int>(token - static_cast<long long>(b) * p.max_len);
+    }
     const int page = t < p.c.lens[b] ? page_of(p.c, b, t) : -1;
     const int in_page = t & ((1 << p.c.page_shift) - 1);
 #pragma unroll
@@ -276,7 +295,7 @@ template <int D>
 int launch_append(const AppendParams& p, bool bf16, bool codes, dim3 grid, cudaStream_t stream) {
   auto kernel = codes ? (bf16 ? paged_append_kernel<D, true, true> : paged_append_kernel<D, false, true>)
                       : (bf16 ? paged_append_kernel<D, true, false> : paged_append_kernel<D, false, false>);
-  return launch_pdl(kernel, grid, dim3(256), 0, stream, p) ? ATTN_B200_OK : ATTN_B200_E_LAUNCH;
+  return launch_pdl(kernel, grid, dim3(kAppendThreads), 0, stream, p) ? ATTN_B200_OK : ATTN_B200_E_LAUNCH;
 }
 
 template <int D>
@@ -320,10 +339,11 @@ int attn_b200_paged_append(const AttnB200PagedAppendArgs* a, void* cuda_stream) 
   p.rot = a->rotary;
   const int sms = device_sms();
   if (sms <= 0) return ATTN_B200_E_LAUNCH;
-  // heads are shared out until two thirds of the chip's threads have work
-  const long long one = rows * (a->cache.head_dim / 16), want = (sms * 1365LL + one - 1) / one;
-  p.lanes = static_cast<int>(std::min<long long>(a->cache.heads_kv, want));
-  const long long blocks = (one * p.lanes + 255) / 256;
+  // heads are shared out evenly until two thirds of the chip's threads have work
+  const long long one = rows * (a->cache.head_dim / 16), want = std::min<long long>(a->cache.heads_kv, (sms * 1365LL + one - 1) / one);
+  const int rounds = static_cast<int>(a->cache.heads_kv / want);
+  p.lanes = (a->cache.heads_kv + rounds - 1) / rounds;
+  const long long blocks = (one * p.lanes + kAppendThreads - 1) / kAppendThreads;
   if (blocks > 0x7fffffff) return ATTN_B200_E_UNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(blocks));
   const bool bf16 = a->dtype == ATTN_B200_DTYPE_BF16;
@@ -347,7 +367,7 @@ int attn_b200_paged_read(const AttnB200PagedReadArgs* a, void* cuda_stream) {
   p.out[1] = static_cast<uint8_t*>(a->v);
   p.max_len = a->max_len;
   p.items = static_cast<long long>(a->cache.batch) * a->max_len * a->cache.heads_kv * (a->cache.head_dim / 16);
-  const long long blocks = std::min<long long>((p.items + 255) / 256, sms * 16LL);
+  const long long blocks = std::min<long long>((p.items + 255) / 256, sms * 64LL);
   const dim3 grid(static_cast<unsigned>(blocks));
   const bool bf16 = a->dtype == ATTN_B200_DTYPE_BF16;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);

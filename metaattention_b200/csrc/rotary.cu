@@ -24,6 +24,8 @@ struct RotaryParams {
   float magnitude;
 };
 
+constexpr int kRotaryThreads = 128;   // of a CTA; 256: 125 us where these take 122 (4 x 4096 x 40 x 128, there and back)
+
 template <class T, int V>
 struct alignas(sizeof(T) * V) Piece {
   T e[V];
@@ -39,7 +41,7 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
 
 // V: values of a piece (a unit is two of them), 16 bytes where dims, strides and addresses are multiples of it, else one value
 template <class T, int V, bool kInterleaved>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
+__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const long long id = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -74,6 +76,19 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
     c0 = unit * V;
     c1 = c0 + p.dim / 2;
   }
+  using P = Piece<T, V>;
+  const long long x_at[2] = {b * p.xs[0][0] + t * p.xs[0][1], b * p.xs[1][0] + t * p.xs[1][1]};
+  const long long y_at[2] = {b * p.ys[0][0] + t * p.ys[0][1], b * p.ys[1][0] + t * p.ys[1][1]};
+  P u, v;
+  auto load = [&](int h, P& u, P& v) {
+    const int w = h < p.heads0 ? 0 : 1;
+    const T* x = static_cast<const T*>(p.x[w]) + x_at[w] + (w == 0 ? h : h - p.heads0) * p.xs[w][2];
+    u = *reinterpret_cast<const P*>(x + c0);
+    if (second) v = *reinterpret_cast<const P*>(x + c1);
+  };
+  // A head is on its way while the angles are made, and the next one while a head is turned: 125 -> 113 us of that case.
+  // (Four heads at once take the registers of half of the warps: 170.)
+  load(lane, u, v);
   float2 cs[V];
   if (turns) {
     long long pos = t;
@@ -84,14 +99,10 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
 #pragma unroll
     for (int i = 0; i < V; ++i) cs[i] = rotary_cos_sin<sizeof(T) == 4>(p.turns[unit * V + i], pos, p.magnitude, p.inverse != 0);
   }
-  using P = Piece<T, V>;
-#pragma unroll 2
+#pragma unroll 1
   for (int h = lane; h < p.heads; h += p.lanes) {
-    const int w = h < p.heads0 ? 0 : 1, hh = w == 0 ? h : h - p.heads0;
-    const T* x = static_cast<const T*>(p.x[w]) + b * p.xs[w][0] + t * p.xs[w][1] + hh * p.xs[w][2];
-    T* y = static_cast<T*>(p.y[w]) + b * p.ys[w][0] + t * p.ys[w][1] + hh * p.ys[w][2];
-    P u = *reinterpret_cast<const P*>(x + c0), v = u;
-    if (second) v = *reinterpret_cast<const P*>(x + c1);
+    P u_next, v_next;
+    if (h + p.lanes < p.heads) load(h + p.lanes, u_next, v_next);
     if (turns) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -103,8 +114,12 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
         c = from_float<T>(fc);
       }
     }
+    const int w = h < p.heads0 ? 0 : 1;
+    T* y = static_cast<T*>(p.y[w]) + y_at[w] + (w == 0 ? h : h - p.heads0) * p.ys[w][2];
     *reinterpret_cast<P*>(y + c0) = u;
     if (second) *reinterpret_cast<P*>(y + c1) = v;
+    u = u_next;
+    v = v_next;
   }
 }
 
@@ -119,10 +134,10 @@ int launch_rotary(RotaryParams& p, bool interleaved, bool copy, long long tokens
   const long long one = tokens * per, want = (sms * 1365LL + one - 1) / one;
   p.lanes = static_cast<int>(std::min<long long>(p.heads, std::max<long long>(want, (p.heads + 9) / 10)));
   p.threads = one * p.lanes;
-  const long long blocks = (p.threads + 255) / 256;
+  const long long blocks = (p.threads + kRotaryThreads - 1) / kRotaryThreads;
   if (blocks > 0x7fffffff) return ATTN_B200_E_UNSUPPORTED;
   auto kernel = interleaved ? rotary_kernel<T, V, true> : rotary_kernel<T, V, false>;
-  return launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p) ? ATTN_B200_OK : ATTN_B200_E_LAUNCH;
+  return launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kRotaryThreads), 0, stream, p) ? ATTN_B200_OK : ATTN_B200_E_LAUNCH;
 }
 
 }  // namespace b200
