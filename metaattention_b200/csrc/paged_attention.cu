@@ -8,82 +8,87 @@ namespace b200 {
 
 // Adds up the partial rows of the units that were cut: o = sum_i exp(lse_i - lse) part_i.  Block x looks after the unit that
 // begins in CTA x and goes on in others, a warp a row.
+constexpr int kMergeRows = 16;   // of a block
+
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ PagedParams p, int ctas) {
   pdl_launch_dependents();
-  const int row = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, c_lo = blockIdx.x;
+  const int lane = threadIdx.x & 31, c_lo = blockIdx.x;
   constexpr int E = D / 32;
   pdl_wait();
-  if (row >= p.rows) return;
   const int4 cut = __ldcg(p.cut + c_lo);
   if (cut.w < 0) return;
-  const int t = row / kPgTile, r = row - t * kPgTile;   // query tile and its row
-  const int g = p.head_major ? r / p.tile_pos : r % p.group, qi = p.head_major ? r % p.tile_pos : r / p.group;
-  if (r >= p.tile_pos * p.group) return;
-  const int tok = cut.z * p.per_tile + t * p.tile_pos + qi, head = cut.y * p.group + g;
-  int row0 = 0, fresh = p.seq;
-  if (p.cu != nullptr) {
-    row0 = min(max(p.cu[cut.x], 0), p.seq);
-    fresh = min(max(p.cu[cut.x + 1], 0), p.seq) - row0;
-  }
-  if (tok >= fresh) return;
-  const int c_hi = min(cut.w, ctas - 1);
-  float mx = -INFINITY, den = 0.0f, acc[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-  // four shares at a time, their statistics and rows loaded together, added up against a running maximum
 #pragma unroll 1
-  for (int c0 = c_lo; c0 <= c_hi; c0 += 4) {
-    float l[4], x[4][E];
+  for (int row = blockIdx.y * kMergeRows + (threadIdx.x >> 5); row < min(p.rows, (static_cast<int>(blockIdx.y) + 1) * kMergeRows); row += 4) {
+    const int t = row / kPgTile, r = row - t * kPgTile;   // query tile and its row
+    const int g = p.head_major ? r / p.tile_pos : r % p.group, qi = p.head_major ? r % p.tile_pos : r / p.group;
+    if (r >= p.tile_pos * p.group) continue;
+    const int tok = cut.z * p.per_tile + t * p.tile_pos + qi, head = cut.y * p.group + g;
+    int row0 = 0, fresh = p.seq;
+    if (p.cu != nullptr) {
+      row0 = min(max(p.cu[cut.x], 0), p.seq);
+      fresh = min(max(p.cu[cut.x + 1], 0), p.seq) - row0;
+    }
+    if (tok >= fresh) continue;
+    const int c_hi = min(cut.w, ctas - 1);
+    float mx = -INFINITY, den = 0.0f, acc[E];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const bool in = c0 + k <= c_hi;
-      const int c = in ? c0 + k : c_hi;
-      const long long slot = (2LL * c + (c == c_lo ? 1 : 0)) * p.rows + row;
-      const float* src = p.part_o + slot * D + lane * E;
-      l[k] = __ldcg(p.part_lse + slot);
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+    // four shares at a time, their statistics and rows loaded together, added up against a running maximum
+#pragma unroll 1
+    for (int c0 = c_lo; c0 <= c_hi; c0 += 4) {
+      float l[4], x[4][E];
 #pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(src + e));
-        x[k][e] = v.x;
-        x[k][e + 1] = v.y;
+      for (int k = 0; k < 4; ++k) {
+        const bool in = c0 + k <= c_hi;
+        const int c = in ? c0 + k : c_hi;
+        const long long slot = (2LL * c + (c == c_lo ? 1 : 0)) * p.rows + row;
+        const float* src = p.part_o + slot * D + lane * E;
+        l[k] = __ldcg(p.part_lse + slot);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(src + e));
+          x[k][e] = v.x;
+          x[k][e + 1] = v.y;
+        }
+        if (!in) l[k] = -INFINITY;
       }
-      if (!in) l[k] = -INFINITY;
+      // shares in which the row saw nothing count nothing; NaN passes through: the maxima ignore it, its weight does not
+      const float m = fmaxf(mx, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])));
+      const float old = mx == -INFINITY ? 0.0f : __expf(mx - m);
+      den *= old;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= old;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const bool in = l[k] != -INFINITY;
+        const float wgt = in ? __expf(l[k] - m) : 0.0f;
+        den += wgt;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = in ? fmaf(wgt, x[k][e], acc[e]) : acc[e];
+      }
+      mx = m;
     }
-    // shares in which the row saw nothing count nothing; NaN passes through: the maxima ignore it, its weight does not
-    const float m = fmaxf(mx, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])));
-    const float old = mx == -INFINITY ? 0.0f : __expf(mx - m);
-    den *= old;
+    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+    const long long at = row0 + tok;
+    uint16_t* orow = static_cast<uint16_t*>(p.o) + (p.cu != nullptr ? 0 : cut.x * p.o_sb) + at * p.o_ss + head * p.o_sh + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] *= old;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const bool in = l[k] != -INFINITY;
-      const float wgt = in ? __expf(l[k] - m) : 0.0f;
-      den += wgt;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = in ? fmaf(wgt, x[k][e], acc[e]) : acc[e];
-    }
-    mx = m;
+    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(orow + e) = pack2<kBf16>(acc[e] * inv, acc[e + 1] * inv);
+    if (lane == 0 && p.lse != nullptr)
+      p.lse[(p.cu != nullptr ? static_cast<long long>(head) : static_cast<long long>(cut.x) * p.heads + head) * p.seq + at] = den == 0.0f ? -INFINITY : mx + logf(den);
   }
-  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-  const long long at = row0 + tok;
-  uint16_t* orow = static_cast<uint16_t*>(p.o) + (p.cu != nullptr ? 0 : cut.x * p.o_sb) + at * p.o_ss + head * p.o_sh + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(orow + e) = pack2<kBf16>(acc[e] * inv, acc[e + 1] * inv);
-  if (lane == 0 && p.lse != nullptr)
-    p.lse[(p.cu != nullptr ? static_cast<long long>(head) : static_cast<long long>(cut.x) * p.heads + head) * p.seq + at] = den == 0.0f ? -INFINITY : mx + logf(den);
 }
 
 int paged_merge(const AttnB200PagedAttnArgs* a, const PagedPlan& d, const PagedParams& p, cudaStream_t stream) {
-  if (d.ctas == 1) return ATTN_B200_OK;   // one share: nothing was cut
+  if (d.ctas == 1 || d.whole) return ATTN_B200_OK;   // nothing was cut
   const bool bf16 = a->dtype == ATTN_B200_DTYPE_BF16;
   auto kernel = a->cache.head_dim == 64 ? (bf16 ? paged_merge_kernel<64, true> : paged_merge_kernel<64, false>)
                                         : (bf16 ? paged_merge_kernel<128, true> : paged_merge_kernel<128, false>);
-  return launch_pdl(kernel, dim3(d.ctas, (d.rows + 3) / 4), dim3(128), 0, stream, p, d.ctas) ? ATTN_B200_OK : ATTN_B200_E_LAUNCH;
+  return launch_pdl(kernel, dim3(d.ctas, (d.rows + kMergeRows - 1) / kMergeRows), dim3(128), 0, stream, p, d.ctas) ? ATTN_B200_OK : ATTN_B200_E_LAUNCH;
 }
 
-constexpr int kPgFew = 32;   // rows of a unit of paged_tokens.cu
+constexpr int kPgFew = 32;       // rows of a unit of paged_tokens.cu
+constexpr int kPgWholeTiles = 4; // KV tiles of a unit that is not cut: the merge behind it costs 3 us, a tile 0.8
 
 inline int plan_paged(const AttnB200PagedAttnArgs* a, int sms, PagedPlan* d) {
   const AttnB200PagedCache& c = a->cache;
@@ -100,17 +105,23 @@ inline int plan_paged(const AttnB200PagedAttnArgs* a, int sms, PagedPlan* d) {
   // A few rows a sequence: their own kernel.  How many a packed sequence has the host does not know; where they are less than
   // two on average a longer one among them costs a walk over its keys for each kPgFew of its rows.
   d->few = d->group <= kPgFew && (packed ? a->seq < 2LL * c.batch : static_cast<long long>(d->group) * a->seq <= kPgFew);
-  d->tile_pos = std::min((d->few ? kPgFew : kPgTile) / d->group, a->seq);
+  // packed tokens, most of them alone: the narrower score tile
+  const int most_rows = !d->few ? kPgTile : packed && d->group <= kPgFew / 2 ? kPgFew / 2 : kPgFew;
+  d->tile_pos = std::min(most_rows / d->group, a->seq);
   d->per_tile = d->few || a->seq <= d->tile_pos ? d->tile_pos : 2 * d->tile_pos;
   d->rows = (d->per_tile > d->tile_pos ? kPgTile : 0) + d->tile_pos * d->group;
   const long long most_kv = static_cast<long long>(c.max_blocks) * c.page_size;
   if (most_kv > 0x3fffffff) return ATTN_B200_E_UNSUPPORTED;
   const long long q_tiles = packed ? a->seq / d->per_tile + c.batch : static_cast<long long>(c.batch) * ((a->seq + d->per_tile - 1) / d->per_tile);
-  const long long most = q_tiles * c.heads_kv * ((most_kv + kPgTile - 1) / kPgTile);
+  long long unit_tiles = (most_kv + kPgTile - 1) / kPgTile;   // at most
+  if (a->window > 0) unit_tiles = std::min<long long>(unit_tiles, (static_cast<long long>(a->window) + d->per_tile - 2) / kPgTile + 2);
+  d->whole = unit_tiles <= kPgWholeTiles;
+  const long long most = q_tiles * c.heads_kv * (d->whole ? 1 : unit_tiles);
   if (most > 0x3fffffff) return ATTN_B200_E_UNSUPPORTED;
   d->ctas = static_cast<int>(std::min<long long>(sms, most));
-  d->off_lse = 2LL * d->ctas * d->rows * c.head_dim * 4;
-  d->off_cut = (d->off_lse + 2LL * d->ctas * d->rows * 4 + 15) / 16 * 16;
+  const long long parts = d->whole ? 0 : 2LL * d->ctas * d->rows;
+  d->off_lse = parts * c.head_dim * 4;
+  d->off_cut = (d->off_lse + parts * 4 + 15) / 16 * 16;
   d->bytes = (d->off_cut + 16LL * d->ctas + 255) / 256 * 256;
   return ATTN_B200_OK;
 }
@@ -209,6 +220,7 @@ int paged_setup(const AttnB200PagedAttnArgs* a, const PagedPlan& d, int* status,
   while ((1 << p.box_shift) < box) ++p.box_shift;
   p.causal = a->causal != 0;
   p.window = a->window;
+  p.whole = d.whole ? 1 : 0;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   p.part_o = reinterpret_cast<float*>(ws);
   p.part_lse = reinterpret_cast<float*>(ws + d.off_lse);

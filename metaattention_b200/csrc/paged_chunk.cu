@@ -26,14 +26,15 @@ struct ChunkSmem {
   static constexpr int kStagesK = D == 128 ? 2 : 4, kStagesV = D == 128 ? (k8Bit ? 1 : 2) : 4;
   static constexpr int kRawK = k8Bit ? (D == 128 ? 2 : 3) : 0, kRawV = k8Bit ? (D == 128 ? 1 : 2) : 0;   // tiles of codes
   static constexpr int kScales = k8Bit ? 4 : 0;                      // tiles of exponents
+  static constexpr int kQBufs = D == 64 && !k8Bit ? 2 : 1;                     // units whose queries are there
   static constexpr int kOffQ = 0;
-  static constexpr int kOffK = kOffQ + 2 * kTileBytes;
+  static constexpr int kOffK = kOffQ + kQBufs * 2 * kTileBytes;
   static constexpr int kOffV = kOffK + kStagesK * kTileBytes;
   static constexpr int kOffRawK = kOffV + kStagesV * kTileBytes;
   static constexpr int kOffRawV = kOffRawK + kRawK * kRawBytes;
   static constexpr int kOffScales = kOffRawV + kRawV * kRawBytes;    // uint8 [kScales][2][128]
   static constexpr int kOffBar = kOffScales + kScales * 2 * kPgTile;
-  static constexpr int kQFull = 0, kQEmpty = 1, kSFull = 2, kPReady = 4, kODone = 6, kOFree = 8, kKFull = 10, kKEmpty = kKFull + kStagesK;
+  static constexpr int kQFull = 0, kQEmpty = 2, kSFull = 4, kPReady = 6, kODone = 8, kOFree = 10, kKFull = 12, kKEmpty = kKFull + kStagesK;
   static constexpr int kVFull = kKEmpty + kStagesK, kVEmpty = kVFull + kStagesV, kRawKFull = kVEmpty + kStagesV, kRawKEmpty = kRawKFull + kRawK;
   static constexpr int kRawVFull = kRawKEmpty + kRawK, kRawVEmpty = kRawVFull + kRawV, kScFull = kRawVEmpty + kRawV, kScEmpty = kScFull + kScales;
   static constexpr int kSFree = kScEmpty + kScales, kNumBars = kSFree + 2;   // the scores of a buffer are in registers
@@ -126,14 +127,15 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
     paged_load<k8Bit ? 1 : KC, k8Bit ? D : 128, k8Bit ? L::kRawK : L::kStagesK>(
         p, make_walk(), &maps.k, p.ok, k8Bit ? smem + L::kOffRawK : sK, k8Bit ? L::kRawBytes : L::kTileBytes, kChunk, bars + (k8Bit ? L::kRawKFull : L::kKFull),
         bars + (k8Bit ? L::kRawKEmpty : L::kKEmpty), ab, kPgKEmpty, [&](const PagedWalk& u, int ui) -> bool {
-          if (ui > 0 && !warp_all(paged_wait(bars + L::kQEmpty, (ui - 1) & 1, ab, kPgQEmpty))) return false;
+          const int qb = ui % L::kQBufs;
+          if (ui >= L::kQBufs && !warp_all(paged_wait(bars + L::kQEmpty + qb, (ui / L::kQBufs - 1) & 1, ab, kPgQEmpty))) return false;
           if (lane == 0) {
             const int tiles = p.per_tile > p.tile_pos ? 2 : 1;
-            mbar_arrive_expect_tx(bars + L::kQFull, tiles * KC * p.tile_pos * p.group * 128);
+            mbar_arrive_expect_tx(bars + L::kQFull + qb, tiles * KC * p.tile_pos * p.group * 128);
             const int s = (p.cu != nullptr ? tab.row[u.b] : 0) + u.qt * p.per_tile;
             for (int t = 0; t < tiles; ++t)
               for (int c = 0; c < KC; ++c)
-                tma_load_rows(sQ + t * L::kTileBytes + c * kChunk, &maps.q, bars + L::kQFull, c * 64, s + t * p.tile_pos, u.h * p.group, p.cu != nullptr ? 0 : u.b, p.oq);
+                tma_load_rows(sQ + (qb * 2 + t) * L::kTileBytes + c * kChunk, &maps.q, bars + L::kQFull + qb, c * 64, s + t * p.tile_pos, u.h * p.group, p.cu != nullptr ? 0 : u.b, p.oq);
           }
           return true;
         });
@@ -156,7 +158,8 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
         int begin[2], end[2];
         keys_of(u, 0, begin[0], end[0]);
         keys_of(u, 1, begin[1], end[1]);
-        ok = wait(bars + L::kQFull, ui & 1, kPgQFull);
+        const int qb = ui % L::kQBufs;
+        ok = wait(bars + L::kQFull + qb, (ui / L::kQBufs) & 1, kPgQFull);
         for (int i = 0; i < u.n && ok; ++i) {
           const int kv0 = (u.lo + u.t0 + i) * N;
           ok = wait(bars + L::kKFull + st, par, kPgKFull);
@@ -172,7 +175,7 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
             }
             if (!ok) continue;
             tc_fence_after_sync();
-            const uint64_t a = q_desc0 + static_cast<uint64_t>(t * (L::kTileBytes >> 4));
+            const uint64_t a = q_desc0 + static_cast<uint64_t>((qb * 2 + t) * (L::kTileBytes >> 4));
             if (elect_one()) {
 #pragma unroll
               for (int ch = 0; ch < KC; ++ch)
@@ -184,7 +187,7 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
           }
           if (ok && elect_one()) {   // behind the tile's scores, if any
             umma_commit(bars + L::kKEmpty + st);
-            if (i == u.n - 1) umma_commit(bars + L::kQEmpty);
+            if (i == u.n - 1) umma_commit(bars + L::kQEmpty + qb);
           }
           __syncwarp();
           if (++st == L::kStagesK) {
@@ -449,7 +452,8 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
     } else {
       // ======================= K and V in 16 bits, K a tile ahead =======================
       const int ct = tid - 416;
-      const int n = share.t1 - share.t0;
+      int n = 0;   // tiles of the share
+      for (PagedWalk u = make_walk(); u.next();) n += u.n;
       bool ok = true;
       for (int j = 0; j <= n && ok; ++j) {
         if (j < n) {

@@ -5,7 +5,8 @@
 // sequence, so that K and V are read once for the group -- with the 128-row KV tiles that any of its rows sees.  The KV
 // tiles of all units, in order, are cut into one equal share per SM: a long context against a single token is split over the
 // chip, the units of a prompt are spread over it evenly whatever their lengths, and a share walks its units with every ring
-// and barrier phase carried across them.  A unit that lies in one share writes its rows; the others leave fp32 partial rows
+// and barrier phase carried across them.  (Where no unit has more than four tiles, shares are whole units and there is nothing to
+// merge.)  A unit that lies in one share writes its rows; the others leave fp32 partial rows
 // that a second small kernel adds up (paged_attention.cu).  Each CTA counts the list itself from the lengths on the device,
 // so a captured call follows them.
 // Pages are fetched by TMA, a box of up to 128 rows of one page, its index from the block table; boxes without a row that
@@ -41,6 +42,7 @@ struct PagedParams {
   int head_major;                // row = g * per_tile + i (1) or i * group + g (0): the order the tensor map delivers
   int max_blocks, page_shift, pages, box_shift;   // rows of a box: min(page, 128)
   int causal, window;
+  int whole;                     // shares are whole units, not tiles: nothing is cut
   const uint16_t* q;             // 8-bit caches: the queries, and exponents of k and v
   long long qs[3];               // (batch, seq, head)
   const uint8_t* scale8[2];
@@ -93,7 +95,7 @@ struct PagedSpan {
 struct PagedWalk {
   const PagedParams& p;
   const int *cum, *lens, *row0;
-  int t, t_end;
+  int t, t_end;                      // the share, in tiles of the list (whole: in units)
   int b, h, qt, len, fresh, tiles;   // sequence, KV head, query tile; its length, new tokens, query tiles
   int begin, end, lo, total, t0, n;  // keys and KV tiles of the unit; this share's: n from t0 on
   bool started = false;
@@ -111,6 +113,11 @@ struct PagedWalk {
     int rest = t - cum[b];
     h = rest / per_head;
     rest -= h * per_head;
+    t0 = 0;
+    if (p.whole) {
+      qt = rest;
+      return;
+    }
     for (qt = 0;; ++qt) {
       const PagedSpan s(p, len, fresh, qt);
       if (rest < s.n || qt + 1 >= tiles) break;
@@ -142,8 +149,8 @@ struct PagedWalk {
     end = s.end;
     lo = s.lo;
     total = s.n;
-    n = min(total - t0, t_end - t);
-    t += n;
+    n = p.whole ? total : min(total - t0, t_end - t);
+    t += p.whole ? 1 : n;
     return true;
   }
   // rows [a, e) of the unit's i-th tile that any of its rows sees
@@ -188,14 +195,14 @@ struct PagedTables {
     if (p.cu == nullptr && p.seq <= 4 * p.per_tile) {   // a few query tiles: a thread a sequence
       for (int b = tid; b < p.batch; b += threads) {
         int sum = 0;
-        for (int qt = 0; qt * p.per_tile < p.seq; ++qt) sum += PagedSpan(p, len[b], p.seq, qt).n;
+        for (int qt = 0; qt * p.per_tile < p.seq; ++qt) sum += p.whole ? 1 : PagedSpan(p, len[b], p.seq, qt).n;
         cum[b] = sum * p.heads_kv;
       }
     } else {
       for (int b = warp; b < p.batch; b += threads / 32) {
         const int fresh = row[b + 1] - row[b], tiles = (fresh + p.per_tile - 1) / p.per_tile;
         int sum = 0;
-        for (int qt = lane; qt < tiles; qt += 32) sum += PagedSpan(p, len[b], fresh, qt).n;
+        for (int qt = lane; qt < tiles; qt += 32) sum += p.whole ? 1 : PagedSpan(p, len[b], fresh, qt).n;
         if (tiles > 1) {
 #pragma unroll
           for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -500,6 +507,7 @@ __device__ __forceinline__ void paged_widen(const uint8_t* src, const uint8_t* e
 struct PagedPlan {
   int group, per_tile, tile_pos, rows, ctas;
   bool few;          // paged_tokens.cu, else paged_chunk.cu
+  bool whole;        // units are not cut
   long long off_lse, off_cut, bytes;
 };
 
