@@ -8,13 +8,12 @@ operator: its examples take q and k with positions in them.
 from __future__ import annotations
 
 import math
-from fractions import Fraction
 
 import torch
 
 from core.native import lib as native
 
-_TURN = Fraction(2 * math.pi)   # radians of a full turn as the frequencies' own type has them
+_TURN = 2 * math.pi   # radians of a full turn as the frequencies' own type has them
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
@@ -72,7 +71,8 @@ class RotaryEmbedding:
         self.magnitude = m if magnitude is None else float(magnitude)
         if not math.isfinite(self.magnitude):
             raise ValueError(f"magnitude must be finite (got {magnitude})")
-        self._turns = {}   # device index -> the native form
+        self._turns = {}   # device -> the native form
+        self._table = self.turns()
 
     def __getstate__(self):
         """Copies and pickles lay their frequencies out again at their first call."""
@@ -81,19 +81,24 @@ class RotaryEmbedding:
     def turns(self) -> list[int]:
         """The frequencies as 64-bit fractions of a full turn, as signed integers."""
         whole = 1 << 64
-        values = [round(Fraction(x) / _TURN * whole) % whole for x in self.frequencies]
+        top, bottom = _TURN.as_integer_ratio()
+        values = []
+        for x in self.frequencies:
+            n, d = x.as_integer_ratio()
+            n, d = n * bottom * whole, d * top
+            values.append((2 * n + d) // (2 * d) % whole)   # the nearest
         return [x - whole if x >= whole // 2 else x for x in values]
 
     def native_on(self, device: torch.device):
-        index = device.index if device.index is not None else torch.cuda.current_device()
-        made = self._turns.get(index)
+        made = self._turns.get(device)
         if made is None:
+            index = device.index if device.index is not None else torch.cuda.current_device()
             if torch.cuda.is_current_stream_capturing():
                 raise native.NativeError("the first call of a RotaryEmbedding on a device lays its frequencies out there: make it before the capture")
             with torch.inference_mode(False):
-                table = torch.tensor(self.turns(), dtype=torch.int64).to(torch.device("cuda", index))
+                table = torch.tensor(self._table, dtype=torch.int64).to(torch.device("cuda", index))
             torch.cuda.current_stream(index).synchronize()   # other streams use it too
-            made = self._turns[index] = native.host().make_turns(table, self.rotary_dim, self.interleaved, self.magnitude)
+            made = self._turns[device] = native.host().make_turns(table, self.rotary_dim, self.interleaved, self.magnitude)
         return made
 
     def __call__(self, q, k=None, positions=None, inplace: bool = False):
@@ -103,5 +108,5 @@ class RotaryEmbedding:
         once.  Differentiable in q and k (twice too); ``inplace`` writes over q and k instead and keeps no graph."""
         if not q.is_cuda:
             raise native.NativeError("rotary positions need CUDA tensors: there is no CPU path")
-        out = native.host().rotary(self.native_on(q.device), q, k, positions, inplace)
-        return out[0] if k is None else (out[0], out[1])
+        made = self._turns.get(q.device)
+        return native.host().rotary(made if made is not None else self.native_on(q.device), q, k, positions, inplace)

@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/extension.h>
 

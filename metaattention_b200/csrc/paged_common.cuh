@@ -14,6 +14,8 @@
 // shared memory (0 * NaN would reach the row), the scores there are masked.
 #pragma once
 
+#include <atomic>
+
 #include <cuda_fp8.h>
 
 #include "../../include/attn_b200.h"
@@ -514,6 +516,21 @@ struct PagedPlan {
 // The launches, by kernel; the tensor maps and parameters of a call are made by paged_setup().
 int launch_paged_tokens(const AttnB200PagedAttnArgs* a, const PagedPlan& d, cudaStream_t stream, int* status);
 int launch_paged_chunk(const AttnB200PagedAttnArgs* a, const PagedPlan& d, cudaStream_t stream, int* status);
+
+// A kernel may have its shared memory: asked for once on each device.
+template <class Kernel>
+inline bool paged_allow(Kernel kernel, int bytes, std::atomic<uint64_t>& asked) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (asked.load(std::memory_order_relaxed) & bit) != 0) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  if (dev < 64) asked.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
 
 struct PagedMaps {
   CUtensorMap q, k, v;

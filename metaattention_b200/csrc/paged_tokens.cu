@@ -513,10 +513,8 @@ int launch_tokens(const AttnB200PagedAttnArgs* a, const PagedPlan& d, cudaStream
   const int rc = paged_setup(a, d, status, &p, &maps);
   if (rc != ATTN_B200_OK) return rc;
   auto kernel = paged_tokens_kernel<D, R, kBf16, k8Bit>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != cudaSuccess) {
-    cudaGetLastError();
-    return ATTN_B200_E_LAUNCH;
-  }
+  static std::atomic<uint64_t> asked{0};
+  if (!paged_allow(kernel, L::kBytes, asked)) return ATTN_B200_E_LAUNCH;
   return launch_pdl(kernel, dim3(d.ctas), dim3(L::kThreads), L::kBytes, stream, maps, p) ? paged_merge(a, d, p, stream) : ATTN_B200_E_LAUNCH;
 }
 
