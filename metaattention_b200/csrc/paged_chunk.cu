@@ -275,8 +275,11 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
       float rs[2];
       F::init(rs, ctx);
       bool begun = false;
+      // the walk waits in memory: its registers belong to the row's scores
+      const int kv_first = (u.lo + u.t0) * N, kv_last = kv_first + u.n * N;
+      asm volatile("" ::"l"(&u) : "memory");
 #pragma unroll 1
-      for (int kv0 = (u.lo + u.t0) * N, kv1 = kv0 + u.n * N; kv0 < kv1; kv0 += N) {
+      for (int kv0 = kv_first; kv0 < kv_last; kv0 += N) {
         if (kv0 >= end || kv0 + N <= begin) continue;
         paged_wait(bars + L::kSFull + t, own & 1, ab, kPgSFull);
         ++own;
@@ -303,10 +306,16 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive(bars + L::kSFree + (L::kScores == 2 ? t : 0));
-          if (edge) {
+          if (edge) {   // mostly on one side
             const int e1 = e - half * TC, a1 = a - half * TC;
+            if (__any_sync(0xffffffffu, e1 < TC)) {
 #pragma unroll
-            for (int k = 0; k < TC; ++k) s[k] = k < e1 && k >= a1 ? s[k] : -INFINITY;
+              for (int k = 0; k < TC; ++k) s[k] = k < e1 ? s[k] : -INFINITY;
+            }
+            if (__any_sync(0xffffffffu, a1 > 0)) {
+#pragma unroll
+              for (int k = 0; k < TC; ++k) s[k] = k >= a1 ? s[k] : -INFINITY;
+            }
           }
           o_scale = F::template tile_pieces<TC, TC / 32>(s, rs, ctx, [&](float mx) { return fmaxf(mx, exchange(mx)); }, [&](int c) {
             if (c == 0 && begun) {   // P's columns are free, and the accumulator is, behind the tile's last P.V
