@@ -282,7 +282,10 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
       float acc[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) acc[r] = 0.0f;
-      for (int i = (J0 ^ group) & 1; i < u.n; i += 2) {
+      const int n = u.n, kv_first = (u.lo + u.t0) * N, end = u.end;
+      if constexpr (k8Bit) asm volatile("" ::"l"(&u) : "memory");   // the walk waits in memory
+#pragma unroll 1
+      for (int i = (J0 ^ group) & 1; i < n; i += 2) {
         const int J = J0 + i, sb = J % L::kScores;
         paged_wait(bars + L::kSFull + sb, (J / L::kScores) & 1, ab, kPgSFull);
         tc_fence_after_sync();
@@ -315,13 +318,13 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
             s[r] *= c2;
           }
         }
-        const int kv0 = (u.lo + u.t0 + i) * N, key = kv0 + key0;
+        const int kv0 = kv_first + i * N, key = kv0 + key0;
         if (kv0 < all_begin || kv0 + N > all_end) {
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             if (r % 4 == 0 && r >= p.rows) break;
             const int pos = first + s_pos[r];
-            const bool in = key < u.end && (!p.causal || key <= pos) && (p.window == 0 || key > pos - p.window);
+            const bool in = key < end && (!p.causal || key <= pos) && (p.window == 0 || key > pos - p.window);
             s[r] = in ? s[r] : -INFINITY;
           }
         }
