@@ -175,7 +175,9 @@ struct PagedTables {
     for (int b = tid; b <= p.batch; b += threads) {
       row[b] = p.cu != nullptr ? min(max(p.cu[b], 0), p.seq) : b * p.seq;
       if (b < p.batch) len[b] = min(max(p.lens[b], 0), most);
+      if (p.whole) cum[b] = b * (p.heads_kv * ((p.seq + p.per_tile - 1) / p.per_tile));   // units: the same for every sequence, unless packed
     }
+    if (p.whole && p.cu == nullptr) return;
     __syncthreads();
     if (p.cu != nullptr) {   // first rows that go backwards count as their predecessors: no row is two sequences'
       if (warp == 0) {

@@ -41,9 +41,10 @@ struct TokensSmem {
   static constexpr int kOffRaw = kOffV + kStagesV * kTileBytes;
   static constexpr int kOffScales = kOffRaw + kRaw * kRawBytes;      // uint8 [kScales][2][128]
   static constexpr int kOffQs = kOffScales + kScales * 2 * kPgTile;   // float [4][R]: factors of the query rows, by unit
-  // float [2][2][R] by unit and group: reference maxima, and sums; float [2][R] by group: rescales; int [R]: positions in the tile
+  // float [2][2][R] by unit and group: reference maxima, and sums; float [2][R] by group: rescales; int [2][R]: position in the
+  // tile and head of the group of each row
   static constexpr int kOffRow = kOffQs + (k8Bit ? 4 * R * 4 : 0);
-  static constexpr int kOffWarp = kOffRow + 11 * R * 4;              // float [8][R]: a value of each warp
+  static constexpr int kOffWarp = kOffRow + 12 * R * 4;              // float [8][R]: a value of each warp
   static constexpr int kOffBar = kOffWarp + 8 * R * 4;
   static constexpr int kQFull = 0, kQEmpty = 2, kPReady = 4, kODone = 6, kOFree = 8, kSFull = 10, kSFree = kSFull + kScores, kKFull = kSFree + kScores;
   static constexpr int kKEmpty = kKFull + kStagesK, kVFull = kKEmpty + kStagesK, kVEmpty = kVFull + kStagesV;
@@ -91,6 +92,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
   float* s_sums = s_refs + 4 * R;
   float* s_rescales = s_sums + 4 * R;
   int* s_pos = reinterpret_cast<int*>(s_rescales + 2 * R);
+  int* s_head = s_pos + R;
   float* s_warps = reinterpret_cast<float*>(smem + L::kOffWarp);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
@@ -132,7 +134,10 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
     for (int i = tid; i < 2 * L::kQBytes / 16; i += L::kThreads) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
     fence_proxy_async_smem();
   }
-  if (tid < R) s_pos[tid] = p.head_major ? tid % p.per_tile : tid / p.group;
+  if (tid < R) {
+    s_pos[tid] = p.head_major ? tid % p.per_tile : tid / p.group;
+    s_head[tid] = p.head_major ? tid / p.per_tile : tid % p.group;
+  }
   pdl_wait();
   if (tid == 0) {
     *abort_flag = (*reinterpret_cast<volatile int*>(p.status) != 0) ? 1 : 0;
@@ -434,7 +439,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
           const float sum = sum0[r] * w0 + sum0[R + r] * w1, inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // no key: 0, and -inf
           // an accumulator that the unit has not used holds anything
           const float v = ((has0 ? x[k] * w0 : 0.0f) + (has1 ? y[k] * w1 : 0.0f)) * inv;
-          const int head = u.h * p.group + (p.head_major ? r / p.per_tile : r - s_pos[r] * p.group);
+          const int head = u.h * p.group + s_head[r];
           if (whole) {
             const uint32_t two = pack2<kBf16>(v, 0.0f);
             o[(row0 + tok) * p.o_ss + head * p.o_sh] = static_cast<uint16_t>(two);
@@ -449,7 +454,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
           const float m = fmaxf(ref0[tid], ref0[R + tid]);
           const float sum = sum0[tid] * fast_exp2(ref0[tid] - m) + sum0[R + tid] * fast_exp2(ref0[R + tid] - m);
           const float lse = sum == 0.0f ? -INFINITY : logf(sum) + m * 0.6931471805599453f;
-          const int head = u.h * p.group + (p.head_major ? tid / p.per_tile : tid - s_pos[tid] * p.group);
+          const int head = u.h * p.group + s_head[tid];
           if (!whole) p.part_lse[slot + tid] = lse;
           else if (p.lse != nullptr) p.lse[(p.cu != nullptr ? static_cast<long long>(head) : static_cast<long long>(u.b) * p.heads + head) * p.seq + row0 + tok] = lse;
         }
