@@ -92,7 +92,6 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
   float* s_sums = s_refs + 4 * R;
   float* s_rescales = s_sums + 4 * R;
   int* s_pos = reinterpret_cast<int*>(s_rescales + 2 * R);
-  int* s_head = s_pos + R;
   float* s_warps = reinterpret_cast<float*>(smem + L::kOffWarp);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
@@ -136,7 +135,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
   }
   if (tid < R) {
     s_pos[tid] = p.head_major ? tid % p.per_tile : tid / p.group;
-    s_head[tid] = p.head_major ? tid / p.per_tile : tid % p.group;
+    if (!k8Bit) s_pos[R + tid] = p.head_major ? tid / p.per_tile : tid % p.group;
   }
   pdl_wait();
   if (tid == 0) {
@@ -270,6 +269,9 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
     const uint32_t line = smem_u32(sP) + group * L::kPBytes + (key0 >> 6) * (R * 128) + (key0 & 7) * 2, p_piece = (key0 >> 3) & 7;
     float *s_rescale = s_rescales + group * R, *s_warp = s_warps + group * 4 * R;
     auto sync = [&]() { named_sync(1 + group, 128); };
+    auto head_of = [&](const PagedWalk& u, int r) -> int {   // 8 bits: divided, since the table's registers make the loop spill (240 us for 179: 16 sequences, up to 32768 keys)
+      return u.h * p.group + (!k8Bit ? s_pos[R + r] : p.head_major ? r / p.per_tile : r - s_pos[r] * p.group);
+    };
     auto load_rows = [&](uint32_t at, float (&x)[R]) {
       if constexpr (R == 16) tmem_ld16f(at, x);
       else tmem_ld32f(at, x);
@@ -439,7 +441,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
           const float sum = sum0[r] * w0 + sum0[R + r] * w1, inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // no key: 0, and -inf
           // an accumulator that the unit has not used holds anything
           const float v = ((has0 ? x[k] * w0 : 0.0f) + (has1 ? y[k] * w1 : 0.0f)) * inv;
-          const int head = u.h * p.group + s_head[r];
+          const int head = head_of(u, r);
           if (whole) {
             const uint32_t two = pack2<kBf16>(v, 0.0f);
             o[(row0 + tok) * p.o_ss + head * p.o_sh] = static_cast<uint16_t>(two);
@@ -454,7 +456,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
           const float m = fmaxf(ref0[tid], ref0[R + tid]);
           const float sum = sum0[tid] * fast_exp2(ref0[tid] - m) + sum0[R + tid] * fast_exp2(ref0[R + tid] - m);
           const float lse = sum == 0.0f ? -INFINITY : logf(sum) + m * 0.6931471805599453f;
-          const int head = u.h * p.group + s_head[tid];
+          const int head = head_of(u, tid);
           if (!whole) p.part_lse[slot + tid] = lse;
           else if (p.lse != nullptr) p.lse[(p.cu != nullptr ? static_cast<long long>(head) : static_cast<long long>(u.b) * p.heads + head) * p.seq + row0 + tok] = lse;
         }
