@@ -425,6 +425,32 @@ class AttentionEngine:
         return self.attention(*args)
 
     # ------------------------------------------------------------------
+    def paged_attention(self, q, cache, block_table, cache_seqlens, cu_seqlens=None, out=None):
+        """The engine's program for new tokens over a ``PagedKVCache``: its ``attention`` with the scale and the mask that this
+        engine found at construction (like its other calls, a mask is what it was at the lengths of ``qkv_meta``, here between
+        positions of a sequence).  Programs that are softmax attention, with no mask, a causal one or a window that ends at the
+        row's own position; others raise NotImplementedError.  The rows' log-sum-exp is left in ``last_final_rowscales``.  The
+        reference pages MLA decode only (core/template/cute_template_kvshared/flash_api.cpp:61-210)."""
+        if getattr(self, "functor_kind", None) != "builtin_softmax":
+            raise NotImplementedError("a paged cache is read by programs that are softmax attention with a constant scale")
+        if self._sparse_host is not None or self._decode_block is not None:
+            raise NotImplementedError("a paged cache is read with a mask_mod that is causal or a window ending at the row's own position, "
+                                      "and without a block mask")
+        window = None
+        if self.mask_kind == native.MASK_BAND:
+            left, right = self.mask_band
+            if right != 0 or left < 0:
+                raise NotImplementedError(f"a paged cache is read with windows that end at the row's own position (got {left} to the left, "
+                                          f"{right} to the right; {native.MASK_OPEN} is open)")
+            window = left + 1
+        if q.dtype != self.dtype:
+            raise TypeError(f"q is {q.dtype}, the engine was built for {self.dtype}")
+        o, lse = cache.attention(q, block_table, cache_seqlens, cu_seqlens, scale=self._fparams[0],
+                                 causal=self.mask_kind != native.MASK_NONE, window=window, out=out, return_lse=True)
+        self.last_final_rowscales = {self.final_names[0]: lse}
+        return o
+
+    # ------------------------------------------------------------------
     def forward_host(self, q, k, v, *custom, out=None, finals_out=None, batch_chunk=1):
         """Forward pass for q, k, v that live in (pinned) HOST memory: [batch, seq, heads, dim] each.
 

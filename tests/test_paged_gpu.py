@@ -14,6 +14,7 @@ import torch
 
 from attn_engine import PagedKVCache, RotaryEmbedding
 from core.native import lib
+from examples_b200 import programs
 from oracle import paged_math as pm
 
 pytestmark = pytest.mark.gpu
@@ -600,3 +601,89 @@ def test_calls_behind_a_recorded_failure_leave(codes):
     assert lib.last_device_status() == 177
     assert torch.equal(c.cache.attention(q.view(2, 2, 4, 64).cuda(), c.block_table, c.cache_seqlens), o)
     assert lib.last_device_status() == 0
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# layouts and sizes that take the kernels' other paths
+# ---------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hkv", [1, 3])
+@pytest.mark.parametrize("news", [1, 3, 70])
+def test_exponents_that_lie_apart(D, Hkv, news):
+    """Scales with the heads behind the rows, which are read byte by byte; one head of rows of a page is one piece otherwise."""
+    run_attention([news, 150, 400], [news] * 3, 2 * Hkv, Hkv, D, 16, torch.bfloat16, True, seed=21, hnd=False)
+
+
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("H,Hkv,news", [(8, 1, 3), (20, 1, 1), (64, 2, 1), (4, 1, 8), (2, 2, 31)])
+@pytest.mark.parametrize("lens", [[400, 31, 900], [7000]])
+def test_units_of_17_to_32_rows(codes, H, Hkv, news, lens):
+    run_attention(lens, [news] * len(lens), H, Hkv, 128, 64, torch.bfloat16, codes, seed=22)
+    run_attention(lens, [news] * len(lens), H, Hkv, 64, 16, torch.float16, codes, seed=23, window=205)
+
+
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+def test_chunks_over_long_contexts(codes, D):
+    """Units of two tiles of query rows that are cut between SMs, and one sequence alone."""
+    run_attention([4100, 2500], [200, 200], 4, 2, D, 64, torch.bfloat16, codes, seed=24)
+    run_attention([6000], [257], 3, 1, D, 16, torch.float16, codes, seed=25, window=4001)
+    run_attention([6000], [129], 3, 1, D, 16, torch.float16, codes, seed=26, causal=False)
+
+
+@pytest.mark.parametrize("codes", [False, True])
+def test_many_units_of_one_tile(codes):
+    """More units than SMs, none of which is cut: a block takes several, whole."""
+    g = gen(27)
+    lens = torch.randint(1, 400, (90,), generator=g).tolist()
+    run_attention(lens, [1] * 90, 16, 8, 128, 16, torch.bfloat16, codes, seed=27)
+    news = [min(n, 1 + i % 50) for i, n in enumerate(lens)]
+    run_attention(lens, news, 8, 4, 64, 16, torch.float16, codes, packed=True, seed=28)
+
+
+@pytest.mark.parametrize("codes", [False, True])
+def test_pools_of_more_than_2_to_the_31_values(codes):
+    """Pages whose rows lie behind 2^31 values of a pool: written, attended to and read like those of a small one."""
+    page, Hkv, D = 256, 8, 128
+    pages = 2 ** 31 // (page * Hkv * D) + 9
+    lens, news, H = [700, 300], [5, 5], 16
+    dtype = torch.float8_e4m3fn if codes else torch.bfloat16
+    small = PagedKVCache.allocate(8, page, Hkv, D, dtype)
+
+    def pool(of, *shape):
+        big = torch.empty(pages, Hkv, page, *shape, dtype=torch.uint8 if codes else dtype, device="cuda")
+        big[-8:] = of.transpose(1, 2).view(big.dtype)
+        return big.view(of.dtype).transpose(1, 2)
+    sizes = [(small.k, (D,)), (small.v, (D,))] + ([(small.k_scale, ()), (small.v_scale, ())] if codes else [])
+    large = PagedKVCache(*[pool(t, *s) for t, s in sizes])
+    table = torch.tensor([[6, 1, 7], [3, 0, -1]], dtype=torch.int32, device="cuda")
+    seqlens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = []
+    for cache, at in ((small, table), (large, torch.where(table >= 0, table + (pages - 8), table))):
+        for first, n in ((0, 295), (295, 5)):   # the second sequence's tokens; the first's last 295 and 5
+            k, v = (torch.randn(2, n, Hkv, D, generator=gen(31 + first + i)).bfloat16().cuda() for i in range(2))
+            cache.append(k, v, at, seqlens if n == 5 else seqlens - 5)
+        q = torch.randn(2, 5, H, D, generator=gen(40)).bfloat16().cuda()
+        out.append((cache.attention(q, at, seqlens), *cache.read(at, seqlens, 700)))
+    assert lib.last_device_status() == 0
+    assert all(torch.equal(a, b) for a, b in zip(*out)) and bool((out[0][1][0, 405:] != 0).any()) and bool((out[0][0] != 0).any())
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# an engine's program over a cache
+# ---------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("mask,causal,window", [(None, False, None), (programs.causal, True, None), (programs.sliding_window_mask, True, 128)])
+def test_an_engine_reads_a_cache(codes, mask, causal, window):
+    eng = programs.masked_softmax_engine(1, 4, 512, 64, 64, mask)
+    dtype = eng.dtype
+    lens, news = [300, 40, 150], [7, 7, 7]
+    c = Case(lens, 2, 64, 16, dtype, codes, seed=91)
+    q, qd, _ = fresh_rows(news, (4, 64), dtype, False, 92)
+    o = eng.paged_attention(qd, c.cache, c.block_table, c.cache_seqlens)
+    (lse,) = eng.last_final_rowscales.values()
+    check_attention(c, news, q, o, lse, False, 4, causal=causal, window=window, scale=eng._fparams[0])
+    out = torch.empty_like(qd)
+    assert eng.paged_attention(qd, c.cache, c.block_table, c.cache_seqlens, out=out) is not None and torch.equal(out, o)

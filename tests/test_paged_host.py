@@ -14,6 +14,7 @@ import metaattention_b200
 from attn_engine import PagedKVCache, RotaryEmbedding
 from attn_engine.rotary import rotary_frequencies
 from core.native import lib
+from examples_b200 import programs
 from oracle import paged_math as pm
 
 
@@ -189,3 +190,39 @@ def test_null_arguments_are_refused_without_a_gpu(native_lib):
     assert native_lib.attn_b200_paged_workspace_bytes(None) == -1
     import ctypes
     assert native_lib.attn_b200_paged_attention(ctypes.byref(lib.PagedAttnArgs()), None) == -1
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# an engine's program over a cache
+# ---------------------------------------------------------------------------------------------------------------
+
+class Recorder:
+    """Takes the place of a cache and keeps what it is asked."""
+
+    def attention(self, q, *args, **kwargs):
+        self.args, self.kwargs = args, kwargs
+        return "o", "lse"
+
+
+@pytest.mark.parametrize("mask,causal,window", [(None, False, None), (programs.causal, True, None), (programs.sliding_window_mask, True, 128)])
+def test_an_engine_gives_its_scale_and_mask_to_a_cache(mask, causal, window):
+    eng, cache = programs.masked_softmax_engine(1, 2, 300, 64, 64, mask), Recorder()
+    q = torch.zeros(1, 1, 2, 64, dtype=eng.dtype)
+    assert eng.paged_attention(q, cache, "table", "lens", out="out") == "o"
+    assert cache.args == ("table", "lens", None) and cache.kwargs.pop("scale") == pytest.approx(0.125, rel=1e-6)
+    assert cache.kwargs == {"causal": causal, "window": window, "out": "out", "return_lse": True}
+    assert list(eng.last_final_rowscales.values()) == ["lse"]
+
+
+def test_engines_whose_programs_a_cache_does_not_run():
+    q = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16)
+    engines = [programs.masked_softmax_engine(1, 2, 300, 64, 64, lambda b, h, i, j: (i - j < 9) & (j - i < 9)),      # looks ahead
+               programs.masked_softmax_engine(1, 2, 300, 64, 64, lambda b, h, i, j: j >= i),
+               programs.masked_softmax_engine(1, 2, 300, 64, 64, lambda b, h, i, j: (j <= i) & (i // 7 == j // 7)),
+               programs.sparse_decode_engine(1, 2, 2, 300, 64, 64)]
+    for eng in engines:
+        with pytest.raises(NotImplementedError, match="paged"):
+            eng.paged_attention(q, Recorder(), None, None)
+    eng = programs.masked_softmax_engine(1, 2, 300, 64, 64, None)
+    with pytest.raises(TypeError, match="float16"):
+        eng.paged_attention(q.half(), Recorder(), None, None)
