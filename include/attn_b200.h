@@ -449,7 +449,8 @@ int attn_b200_rotary(const AttnB200RotaryArgs* args, void* cuda_stream);
 typedef struct AttnB200PagedCache {
   void* k;                     /* [num_pages, page_size, heads_kv, head_dim] through the strides, last dimension contiguous */
   void* v;
-  uint8_t* k_scale;            /* E4M3: [num_pages, page_size, heads_kv] exponents e; a code stands for code * 2^(e - 127), 255 for NaN */
+  uint8_t* k_scale;            /* E4M3: [num_pages, page_size, heads_kv] exponents e; a code stands for code * 2^(e - 127), a row of
+                                  exponent 255 for NaN; the codes 0x7f and 0xff belong to such rows alone */
   uint8_t* v_scale;
   int64_t k_stride[3];         /* elements of (page, token, head) */
   int64_t v_stride[3];
@@ -465,7 +466,7 @@ typedef struct AttnB200PagedCache {
 
 /* Writes the last tokens of each sequence into the cache.  k, v: [batch, seq, heads_kv, head_dim], or with cu_seqlens
  * (int32 [batch + 1]) packed rows [seq, heads_kv, head_dim] of which cu_seqlens[b] .. cu_seqlens[b + 1] - 1 are the last
- * tokens of sequence b; rows behind cu_seqlens[batch] and tokens at negative positions go nowhere.  E4M3: the scale of a
+ * tokens of sequence b (values that do not decrease); rows behind cu_seqlens[batch] and tokens at negative positions go nowhere.  E4M3: the scale of a
  * row is the least power of two (from 2^-127) that brings its largest magnitude to 448 at most; a row with a value that is
  * not finite is NaN throughout.  `rotary` turns k on its way, in 32 bits and rounded once. */
 typedef struct AttnB200PagedAppendArgs {

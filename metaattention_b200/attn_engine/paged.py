@@ -21,15 +21,16 @@ from core.native import lib as native
 class PagedKVCache:
     """Pools of pages ``k``, ``v`` [num_pages, page_size, heads_kv, head_dim] in float16, bfloat16 or float8_e4m3fn, the last
     with ``k_scale``, ``v_scale`` [num_pages, page_size, heads_kv] (float8_e8m0fnu, or uint8 exponents): a code stands for
-    code * 2^(exponent - 127).  Any strides of whole 16 bytes with a contiguous last dimension; page_size a power of two of at
-    least 8, head_dim 64 or 128.  The pools are the caller's tensors and are written in place.
+    code * 2^(exponent - 127), a row of exponent 255 for NaN; the codes 0x7f and 0xff belong to such rows alone.
+    Any strides of whole 16 bytes with a contiguous last dimension; page_size a power of two of at least 8, head_dim 64 or 128.
+    The pools are the caller's tensors and are written in place.
 
     Common arguments: ``block_table`` int32 [batch, max_blocks] names the page of each page_size tokens of a sequence (entries
     behind its end may hold anything); ``cache_seqlens`` int32 [batch], tokens of each sequence with the new ones among them, at
     most max_blocks * page_size.  New tokens come as [batch, seq, heads, head_dim], the same number for every sequence, or
-    with ``cu_seqlens`` int32 [batch + 1] as packed rows [rows, heads, head_dim], those of sequence b being rows cu_seqlens[b]
-    to cu_seqlens[b + 1] - 1.  Rows behind cu_seqlens[batch] take no part (padding of a captured step).  All of them on the
-    cache's device; calls run on the current stream of that device."""
+    with ``cu_seqlens`` int32 [batch + 1], which do not decrease, as packed rows [rows, heads, head_dim], those of sequence b being
+    rows cu_seqlens[b] to cu_seqlens[b + 1] - 1.  Rows behind cu_seqlens[batch] take no part (padding of a captured step).  All
+    of them on the cache's device; calls run on the current stream of that device."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale

@@ -164,6 +164,7 @@ std::vector<Tensor> rotary_call(const std::shared_ptr<const Turns>& turns, const
     for (const Tensor& t : x)
       for (int64_t d = 0; d < t.dim(); ++d)
         if (t.size(d) > 1 && t.stride(d) == 0) refuse("in place, every value must have memory of its own (an expanded tensor has not)");
+    if (k.has_value() && k->numel() > 0 && k->data_ptr() == q.data_ptr()) refuse("in place, q and k must not be the same memory");
   }
   py::gil_scoped_release others_run;
   c10::cuda::CUDAGuard guard(q.device());
@@ -291,7 +292,7 @@ void cache_append(const Cache& c, const Tensor& k, const Tensor& v, const Tensor
   new_rows(c, k, "k", cu, a.cache.batch, a.cache.heads_kv);
   new_rows(c, v, "v", cu, a.cache.batch, a.cache.heads_kv);
   if (k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type()) refuse("k and v must have the same shape and dtype (got ", shape_of(k), ", ", shape_of(v), ")");
-  if (at::GradMode::is_enabled() && (k.requires_grad() || v.requires_grad())) refuse("a cache has no gradient: append under torch.no_grad()");
+  if (at::GradMode::is_enabled() && (k.requires_grad() || v.requires_grad() || c.k.requires_grad() || c.v.requires_grad())) refuse("a cache has no gradient: append under torch.no_grad()");
   if (turns != nullptr) {
     if (turns->dim % 16 != 0 || turns->dim > c.view.head_dim) refuse("rotary_dim of keys on their way into a cache must be a multiple of 16, up to the head dim");
     if (turns->turns.device() != c.k.device()) refuse("the frequencies are on ", turns->turns.device(), ", the cache is on ", c.k.device());
@@ -318,6 +319,7 @@ std::vector<Tensor> cache_read(const Cache& c, const Tensor& table, const Tensor
   Tensor held;
   a.cache = sequences(c, table, lens, held);
   if (max_len < 0 || max_len > 0x7fffffff) refuse("max_len must not be negative (got ", max_len, ")");
+  if (at::GradMode::is_enabled() && (c.k.requires_grad() || c.v.requires_grad())) refuse("a cache has no gradient: read it under torch.no_grad()");
   if (a.cache.dtype != ATTN_B200_DTYPE_E4M3 && bf16 != (a.cache.dtype == ATTN_B200_DTYPE_BF16)) refuse("a 16-bit cache is read in its own dtype");
   py::gil_scoped_release others_run;
   at::AutoDispatchBelowADInplaceOrView below;
@@ -349,10 +351,13 @@ std::tuple<Tensor, OptTensor> cache_attention(const Cache& c, const Tensor& q, c
   if (!(scale > 0.0) || !std::isfinite(static_cast<float>(scale)) || static_cast<float>(scale) == 0.0f) refuse("scale must be positive and finite (got ", scale, ")");
   if (window < 0) refuse("window must be positive (got ", window, ")");
   if (window > 0 && !causal) refuse("a window counts back from each row: it needs causal=True");
-  if (at::GradMode::is_enabled() && q.requires_grad()) refuse("attention over a paged cache has no backward pass: call it under torch.no_grad()");
+  if (at::GradMode::is_enabled() && (q.requires_grad() || c.k.requires_grad() || c.v.requires_grad() || (out.has_value() && out->requires_grad())))
+    refuse("attention over a paged cache has no backward pass: call it under torch.no_grad()");
   if (out.has_value()) {
     new_rows(c, *out, "out", cu, a.cache.batch, H);
     if (out->sizes() != q.sizes() || out->scalar_type() != q.scalar_type()) refuse("out must have the shape and dtype of q (got ", shape_of(*out), ")");
+    for (int64_t d = 0; d < out->dim(); ++d)
+      if (out->size(d) > 1 && out->stride(d) == 0) refuse("every value of out must have memory of its own (an expanded tensor has not)");
   }
   py::gil_scoped_release others_run;
   at::AutoDispatchBelowADInplaceOrView below;

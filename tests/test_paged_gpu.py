@@ -687,3 +687,24 @@ def test_an_engine_reads_a_cache(codes, mask, causal, window):
     check_attention(c, news, q, o, lse, False, 4, causal=causal, window=window, scale=eng._fparams[0])
     out = torch.empty_like(qd)
     assert eng.paged_attention(qd, c.cache, c.block_table, c.cache_seqlens, out=out) is not None and torch.equal(out, o)
+
+
+def test_memory_that_a_call_must_not_write_is_refused():
+    """Results in memory that several values share, or that a graph holds; pools that want a gradient; q and k turned in one place."""
+    c = Case([20, 30], 2, 64, 16)
+    q = torch.randn(2, 1, 4, 64, dtype=torch.bfloat16, device="cuda")
+    kv = torch.zeros(2, 1, 2, 64, dtype=torch.bfloat16, device="cuda")
+    t, s = c.block_table, c.cache_seqlens
+    for out in (q[:1].expand(2, 1, 4, 64), q.clone().requires_grad_()):
+        with pytest.raises(ValueError):
+            c.cache.attention(q, t, s, out=out)
+    learned = PagedKVCache(c.cache.k.clone().requires_grad_(), c.cache.v.clone())
+    for call in (lambda: learned.attention(q, t, s), lambda: learned.read(t, s, 4), lambda: learned.append(kv, kv, t, s)):
+        with pytest.raises(ValueError, match="no_grad"):
+            call()
+    with torch.no_grad():
+        assert torch.equal(learned.attention(q, t, s), c.cache.attention(q, t, s))
+    with pytest.raises(ValueError, match="same memory"):
+        RotaryEmbedding(64)(q, q, inplace=True)
+    own = q.clone()
+    assert torch.equal(c.cache.attention(own, t, s, out=own), c.cache.attention(q, t, s))   # in q's place
