@@ -7,76 +7,69 @@
 namespace b200 {
 
 // Adds up the partial rows of the units that were cut: o = sum_i exp(lse_i - lse) part_i.  Block x looks after the unit that
-// begins in CTA x and goes on in others, a warp a row.
+// begins in CTA x and goes on in others, a thread 8 columns of a row.
 constexpr int kMergeRows = 16;   // of a block
 
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ PagedParams p, int ctas) {
+__global__ void __launch_bounds__(2 * D) paged_merge_kernel(const __grid_constant__ PagedParams p, int ctas) {
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, c_lo = blockIdx.x;
-  constexpr int E = D / 32;
+  const int c_lo = blockIdx.x, row = blockIdx.y * kMergeRows + threadIdx.x % kMergeRows, col = threadIdx.x / kMergeRows * 8;
+  const int t = row / kPgTile, r = row - t * kPgTile;   // query tile and its row
+  const int g = p.head_major ? r / p.tile_pos : r % p.group, qi = p.head_major ? r % p.tile_pos : r / p.group;
   pdl_wait();
   const int4 cut = __ldcg(p.cut + c_lo);
-  if (cut.w < 0) return;
-#pragma unroll 1
-  for (int row = blockIdx.y * kMergeRows + (threadIdx.x >> 5); row < min(p.rows, (static_cast<int>(blockIdx.y) + 1) * kMergeRows); row += 4) {
-    const int t = row / kPgTile, r = row - t * kPgTile;   // query tile and its row
-    const int g = p.head_major ? r / p.tile_pos : r % p.group, qi = p.head_major ? r % p.tile_pos : r / p.group;
-    if (r >= p.tile_pos * p.group) continue;
-    const int tok = cut.z * p.per_tile + t * p.tile_pos + qi, head = cut.y * p.group + g;
-    int row0 = 0, fresh = p.seq;
-    if (p.cu != nullptr) {
-      row0 = min(max(p.cu[cut.x], 0), p.seq);
-      fresh = min(max(p.cu[cut.x + 1], 0), p.seq) - row0;
-    }
-    if (tok >= fresh) continue;
-    const int c_hi = min(cut.w, ctas - 1);
-    float mx = -INFINITY, den = 0.0f, acc[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    // four shares at a time, their statistics and rows loaded together, added up against a running maximum
-#pragma unroll 1
-    for (int c0 = c_lo; c0 <= c_hi; c0 += 4) {
-      float l[4], x[4][E];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const bool in = c0 + k <= c_hi;
-        const int c = in ? c0 + k : c_hi;
-        const long long slot = (2LL * c + (c == c_lo ? 1 : 0)) * p.rows + row;
-        const float* src = p.part_o + slot * D + lane * E;
-        l[k] = __ldcg(p.part_lse + slot);
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(src + e));
-          x[k][e] = v.x;
-          x[k][e + 1] = v.y;
-        }
-        if (!in) l[k] = -INFINITY;
-      }
-      // shares in which the row saw nothing count nothing; NaN passes through: the maxima ignore it, its weight does not
-      const float m = fmaxf(mx, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])));
-      const float old = mx == -INFINITY ? 0.0f : __expf(mx - m);
-      den *= old;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] *= old;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const bool in = l[k] != -INFINITY;
-        const float wgt = in ? __expf(l[k] - m) : 0.0f;
-        den += wgt;
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = in ? fmaf(wgt, x[k][e], acc[e]) : acc[e];
-      }
-      mx = m;
-    }
-    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-    const long long at = row0 + tok;
-    uint16_t* orow = static_cast<uint16_t*>(p.o) + (p.cu != nullptr ? 0 : cut.x * p.o_sb) + at * p.o_ss + head * p.o_sh + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(orow + e) = pack2<kBf16>(acc[e] * inv, acc[e + 1] * inv);
-    if (lane == 0 && p.lse != nullptr)
-      p.lse[(p.cu != nullptr ? static_cast<long long>(head) : static_cast<long long>(cut.x) * p.heads + head) * p.seq + at] = den == 0.0f ? -INFINITY : mx + logf(den);
+  if (cut.w < 0 || row >= p.rows || r >= p.tile_pos * p.group) return;
+  const int tok = cut.z * p.per_tile + t * p.tile_pos + qi, head = cut.y * p.group + g;
+  int row0 = 0, fresh = p.seq;
+  if (p.cu != nullptr) {
+    row0 = min(max(p.cu[cut.x], 0), p.seq);
+    fresh = min(max(p.cu[cut.x + 1], 0), p.seq) - row0;
   }
+  if (tok >= fresh) return;
+  const int c_hi = min(cut.w, ctas - 1);
+  float mx = -INFINITY, den = 0.0f, acc[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
+  // four shares at a time, their statistics and rows loaded together, added up against a running maximum
+#pragma unroll 1
+  for (int c0 = c_lo; c0 <= c_hi; c0 += 4) {
+    float l[4];
+    float4 x[4][2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool in = c0 + k <= c_hi;
+      const int c = in ? c0 + k : c_hi;
+      const long long slot = (2LL * c + (c == c_lo ? 1 : 0)) * p.rows;
+      const float4* src = reinterpret_cast<const float4*>(p.part_o + slot * D) + col / 4 * p.rows + row;
+      l[k] = __ldcg(p.part_lse + slot + row);
+      x[k][0] = __ldcg(src);
+      x[k][1] = __ldcg(src + p.rows);
+      if (!in) l[k] = -INFINITY;
+    }
+    // shares in which the row saw nothing count nothing; NaN passes through: the maxima ignore it, its weight does not
+    const float m = fmaxf(mx, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])));
+    const float old = mx == -INFINITY ? 0.0f : __expf(mx - m);
+    den *= old;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= old;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (l[k] == -INFINITY) continue;
+      const float wgt = __expf(l[k] - m);
+      const float v[8] = {x[k][0].x, x[k][0].y, x[k][0].z, x[k][0].w, x[k][1].x, x[k][1].y, x[k][1].z, x[k][1].w};
+      den += wgt;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = fmaf(wgt, v[e], acc[e]);
+    }
+    mx = m;
+  }
+  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+  const long long at = row0 + tok;
+  uint16_t* orow = static_cast<uint16_t*>(p.o) + (p.cu != nullptr ? 0 : cut.x * p.o_sb) + at * p.o_ss + head * p.o_sh + col;
+  *reinterpret_cast<uint4*>(orow) = make_uint4(pack2<kBf16>(acc[0] * inv, acc[1] * inv), pack2<kBf16>(acc[2] * inv, acc[3] * inv),
+                                               pack2<kBf16>(acc[4] * inv, acc[5] * inv), pack2<kBf16>(acc[6] * inv, acc[7] * inv));
+  if (col == 0 && p.lse != nullptr)
+    p.lse[(p.cu != nullptr ? static_cast<long long>(head) : static_cast<long long>(cut.x) * p.heads + head) * p.seq + at] = den == 0.0f ? -INFINITY : mx + logf(den);
 }
 
 int paged_merge(const AttnB200PagedAttnArgs* a, const PagedPlan& d, const PagedParams& p, cudaStream_t stream) {
@@ -84,7 +77,7 @@ int paged_merge(const AttnB200PagedAttnArgs* a, const PagedPlan& d, const PagedP
   const bool bf16 = a->dtype == ATTN_B200_DTYPE_BF16;
   auto kernel = a->cache.head_dim == 64 ? (bf16 ? paged_merge_kernel<64, true> : paged_merge_kernel<64, false>)
                                         : (bf16 ? paged_merge_kernel<128, true> : paged_merge_kernel<128, false>);
-  return launch_pdl(kernel, dim3(d.ctas, (d.rows + kMergeRows - 1) / kMergeRows), dim3(128), 0, stream, p, d.ctas) ? ATTN_B200_OK : ATTN_B200_E_LAUNCH;
+  return launch_pdl(kernel, dim3(d.ctas, (d.rows + kMergeRows - 1) / kMergeRows), dim3(2 * a->cache.head_dim), 0, stream, p, d.ctas) ? ATTN_B200_OK : ATTN_B200_E_LAUNCH;
 }
 
 constexpr int kPgFew = 32;       // rows of a unit of paged_tokens.cu

@@ -112,7 +112,7 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
   const uint32_t tmem_base = *tmem_slot;
   const PagedShare share(p, tab);
   const bool run_cta = warp_all(share.t1 > share.t0 && !*abort_flag);
-  auto make_walk = [&]() { return PagedWalk(p, tab.cum, tab.len, tab.row, share.t0, share.t1); };
+  auto make_walk = [&]() { return PagedWalk(p, tab.cum, tab.len, tab.row, tab.start, share.t0, share.t1); };
   // keys [begin, end) that any row of the unit's query tile t sees
   auto keys_of = [&](const PagedWalk& u, int t, int& begin, int& end) {
     const int tok = u.qt * p.per_tile + t * p.tile_pos, n = min(p.tile_pos, u.fresh - tok);   // the tile's tokens
@@ -407,7 +407,7 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
       const int head = u.h * p.group + g;
       const bool whole = u.n == u.total;
       // a partial result: the unit's first share leaves it in the second slot of its CTA, the later ones in the first
-      const long long slot = (2LL * cta + (u.t0 == 0 ? 1 : 0)) * p.rows + t * N + row;
+      const long long slot = (2LL * cta + (u.t0 == 0 ? 1 : 0)) * p.rows;
       const long long at = p.cu != nullptr ? tab.row[u.b] + tok : tok;   // row of o
       uint16_t* orow = static_cast<uint16_t*>(p.o) + (p.cu != nullptr ? 0 : u.b * p.o_sb) + at * p.o_ss + head * p.o_sh + half * OC;
       if (any_live) {
@@ -438,14 +438,14 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
                 reinterpret_cast<uint4*>(orow + c * 32)[v] = pk;
               }
             } else {
-              float4* dst = reinterpret_cast<float4*>(p.part_o + slot * D + half * OC + c * 32);
+              float4* dst = reinterpret_cast<float4*>(p.part_o + slot * D) + (half * (OC / 4) + c * 8) * p.rows + t * N + row;
 #pragma unroll
-              for (int v = 0; v < 8; ++v) dst[v] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+              for (int v = 0; v < 8; ++v) dst[v * p.rows] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
             }
           }
         }
         if (live && half == 0) {
-          if (!whole) p.part_lse[slot] = lse;
+          if (!whole) p.part_lse[slot + t * N + row] = lse;
           else if (p.lse != nullptr) p.lse[(p.cu != nullptr ? static_cast<long long>(head) : static_cast<long long>(u.b) * p.heads + head) * p.seq + at] = lse;
         }
       }

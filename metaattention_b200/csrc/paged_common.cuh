@@ -49,7 +49,7 @@ struct PagedParams {
   long long qs[3];               // (batch, seq, head)
   const uint8_t* scale8[2];
   long long scale_stride[2][3];
-  float* part_o;                 // [2 * CTAs][rows][D]
+  float* part_o;                 // [2 * CTAs][D / 4][rows][4]: in paged_chunk.cu a lane has a row (a row's columns in one piece: 4100 cycles a unit)
   float* part_lse;               // [2 * CTAs][rows]
   int4* cut;                     // [CTAs] sequence, KV head, query tile and last CTA of the unit that begins in a CTA and goes on, or w = -1
   CoordOrder oq, ok, ov;
@@ -101,31 +101,14 @@ struct PagedWalk {
   int b, h, qt, len, fresh, tiles;   // sequence, KV head, query tile; its length, new tokens, query tiles
   int begin, end, lo, total, t0, n;  // keys and KV tiles of the unit; this share's: n from t0 on
   bool started = false;
-  __device__ PagedWalk(const PagedParams& p_, const int* cum_, const int* lens_, const int* row0_, int t_, int t_end_)
+  __device__ PagedWalk(const PagedParams& p_, const int* cum_, const int* lens_, const int* row0_, const int* start, int t_, int t_end_)
       : p(p_), cum(cum_), lens(lens_), row0(row0_), t(t_), t_end(t_end_) {
     if (t >= t_end) return;
-    int a = 0, z = p.batch;   // last sequence with cum[b] <= t: it has tiles
-    while (z - a > 1) {
-      const int mid = (a + z) >> 1;
-      if (cum[mid] <= t) a = mid; else z = mid;
-    }
-    b = a;
+    b = start[0];
+    h = start[1];
+    qt = start[2];
+    t0 = start[3];
     sequence();
-    const int per_head = (cum[b + 1] - cum[b]) / p.heads_kv;
-    int rest = t - cum[b];
-    h = rest / per_head;
-    rest -= h * per_head;
-    t0 = 0;
-    if (p.whole) {
-      qt = rest;
-      return;
-    }
-    for (qt = 0;; ++qt) {
-      const PagedSpan s(p, len, fresh, qt);
-      if (rest < s.n || qt + 1 >= tiles) break;
-      rest -= s.n;
-    }
-    t0 = rest;
   }
   __device__ void sequence() {
     len = lens[b];
@@ -163,11 +146,57 @@ struct PagedWalk {
   }
 };
 
-// Lengths, first rows of the new tokens and tiles in front of every sequence, by all `threads` of the CTA; the caller syncs behind it.
+// Lengths, first rows of the new tokens and tiles in front of every sequence, by all `threads` of the CTA, and the place in the list
+// where its share begins, by one warp (each role's warps looking for it themselves ran the same cold code six times over: 6500 cycles in
+// front of a chunk's first unit, 3000 with this); the caller syncs behind it.
 struct PagedTables {
   int *cum, *len, *row;   // [batch + 1], [batch], [batch + 1] in shared memory
-  static constexpr int kBytes = (3 * kPgMaxBatch + 2) * 4;
-  __device__ explicit PagedTables(uint8_t* at) : cum(reinterpret_cast<int*>(at)), len(cum + kPgMaxBatch + 1), row(len + kPgMaxBatch) {}
+  int* start;             // sequence, KV head, query tile and tile of that unit
+  static constexpr int kBytes = (3 * kPgMaxBatch + 6) * 4;
+  __device__ explicit PagedTables(uint8_t* at)
+      : cum(reinterpret_cast<int*>(at)), len(cum + kPgMaxBatch + 1), row(len + kPgMaxBatch), start(row + kPgMaxBatch + 1) {}
+
+  __device__ void locate(const PagedParams& p) const {   // by a warp
+    const int lane = threadIdx.x & 31, total = cum[p.batch], shares = min(static_cast<int>(gridDim.x), total);
+    if (static_cast<int>(blockIdx.x) >= shares) return;
+    const int t = pg_share(total, blockIdx.x, shares);
+    int b = 0;   // last sequence with cum[b] <= t: it has tiles
+    for (int i0 = 0; i0 < p.batch; i0 += 32) {
+      const uint32_t in = __ballot_sync(0xffffffffu, i0 + lane < p.batch && cum[i0 + lane] <= t);
+      if (in == 0) break;
+      b = i0 + 31 - __clz(in);
+    }
+    const int per_head = (cum[b + 1] - cum[b]) / p.heads_kv, h = (t - cum[b]) / per_head;
+    int rest = t - cum[b] - h * per_head, qt = rest;
+    if (p.whole) {
+      rest = 0;
+    } else {
+      const int fresh = row[b + 1] - row[b], tiles = (fresh + p.per_tile - 1) / p.per_tile;
+      for (int q0 = 0; q0 < tiles; q0 += 32) {
+        const int n = q0 + lane < tiles ? PagedSpan(p, len[b], fresh, q0 + lane).n : 0;
+        int x = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, d);
+          if (lane >= d) x += y;
+        }
+        const uint32_t behind = __ballot_sync(0xffffffffu, x > rest);
+        if (behind != 0) {
+          const int at = __ffs(behind) - 1;
+          qt = q0 + at;
+          rest -= __shfl_sync(0xffffffffu, x - n, at);
+          break;
+        }
+        rest -= __shfl_sync(0xffffffffu, x, 31);
+      }
+    }
+    if (lane == 0) {
+      start[0] = b;
+      start[1] = h;
+      start[2] = qt;
+      start[3] = rest;
+    }
+  }
 
   __device__ void count(const PagedParams& p, int threads) const {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -177,8 +206,11 @@ struct PagedTables {
       if (b < p.batch) len[b] = min(max(p.lens[b], 0), most);
       if (p.whole) cum[b] = b * (p.heads_kv * ((p.seq + p.per_tile - 1) / p.per_tile));   // units: the same for every sequence, unless packed
     }
-    if (p.whole && p.cu == nullptr) return;
     __syncthreads();
+    if (p.whole && p.cu == nullptr) {
+      if (warp == 0) locate(p);
+      return;
+    }
     if (p.cu != nullptr) {   // first rows that go backwards count as their predecessors: no row is two sequences'
       if (warp == 0) {
         int run = 0;
@@ -229,6 +261,8 @@ struct PagedTables {
         run += __shfl_sync(0xffffffffu, x, 31);
       }
       if (lane == 0) cum[p.batch] = run;
+      __syncwarp();
+      locate(p);
     }
   }
 };

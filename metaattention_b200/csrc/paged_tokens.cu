@@ -153,7 +153,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
   const uint32_t tmem_base = *tmem_slot;
   const PagedShare share(p, tab);
   const bool run_cta = warp_all(share.t1 > share.t0 && !*abort_flag);
-  auto make_walk = [&]() { return PagedWalk(p, tab.cum, tab.len, tab.row, share.t0, share.t1); };
+  auto make_walk = [&]() { return PagedWalk(p, tab.cum, tab.len, tab.row, tab.start, share.t0, share.t1); };
 
   if (!run_cta) {
   } else if (warp == 8) {
@@ -446,7 +446,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
             const uint32_t two = pack2<kBf16>(v, 0.0f);
             o[(row0 + tok) * p.o_ss + head * p.o_sh] = static_cast<uint16_t>(two);
           } else {
-            p.part_o[(slot + r) * D + column] = v;
+            p.part_o[slot * D + ((column >> 2) * p.rows + r) * 4 + (column & 3)] = v;
           }
         }
       }
