@@ -96,6 +96,9 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
+  // head of the group, and position in the tile, of a softmax thread's row
+  const int row_of_tile = (warp & 3) * 32 + lane, by = p.head_major ? p.tile_pos : p.group, high = row_of_tile / by, low = row_of_tile - high * by;
+  const int g = p.head_major ? high : low, qi = p.head_major ? low : high;
   pdl_wait();
   if (tid == 0) {
     *abort_flag = (*reinterpret_cast<volatile int*>(p.status) != 0) ? 1 : 0;
@@ -241,7 +244,7 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
     // ======================= softmax =======================
     constexpr int RT = L::kRowThreads, TC = N / RT, OC = D / RT;   // threads of a row; columns of a thread, of scores and of o
     const int t = warp / (4 * RT), half = RT == 1 ? 0 : (warp >> 2) & 1;
-    const int row = (warp & 3) * 32 + lane;
+    const int row = row_of_tile;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem_base + lane_base + kColS + (L::kScores == 2 ? t * N : 0) + half * TC;
     const uint32_t tP = tmem_base + lane_base + kColP + t * kPStep + half * (TC / 2);
@@ -257,8 +260,6 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
     };
     const FunctorArgs fa{{p.scale}};
     const RowCtx ctx{0, 0, 0, 0, p.seq, 0, &fa};   // softmax asks for the scale only
-    const int g = p.head_major ? row / p.tile_pos : row % p.group;
-    const int qi = p.head_major ? row % p.tile_pos : row / p.group;   // position in the tile
     const float c2 = p.scale * 1.4426950408889634f;
     PagedWalk u = make_walk();
     int own = 0;   // tiles so far

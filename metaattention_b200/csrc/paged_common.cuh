@@ -71,7 +71,11 @@ __device__ __forceinline__ bool paged_wait(uint64_t* bar, uint32_t parity, const
   return mbar_try_wait(bar, parity) || paged_wait_on(bar, parity, ab.cta_flag, ab.device_status, site);
 }
 
-__host__ __device__ __forceinline__ int pg_share(int total, int c, int n) { return static_cast<int>(static_cast<long long>(total) * c / n); }
+// total * c / n, in 32 bits (a division in 64 is 100 instructions, all of them cold)
+__device__ __forceinline__ int pg_share(int total, int c, int n) {
+  const int q = total / n;
+  return q * c + (total - q * n) * c / n;
+}
 __device__ __forceinline__ int pg_owner(int t, int n, int total) { return static_cast<int>((static_cast<long long>(t + 1) * n - 1) / total); }
 
 // Keys [begin, end) that any row of a query tile sees, and the KV tiles they lie in; one (masked) tile where there are none,
@@ -98,7 +102,7 @@ struct PagedWalk {
   const PagedParams& p;
   const int *cum, *lens, *row0;
   int t, t_end;                      // the share, in tiles of the list (whole: in units)
-  int b, h, qt, len, fresh, tiles;   // sequence, KV head, query tile; its length, new tokens, query tiles
+  int b, h, qt, len, fresh;          // sequence, KV head, query tile; its length, new tokens
   int begin, end, lo, total, t0, n;  // keys and KV tiles of the unit; this share's: n from t0 on
   bool started = false;
   __device__ PagedWalk(const PagedParams& p_, const int* cum_, const int* lens_, const int* row0_, const int* start, int t_, int t_end_)
@@ -113,13 +117,12 @@ struct PagedWalk {
   __device__ void sequence() {
     len = lens[b];
     fresh = row0[b + 1] - row0[b];
-    tiles = (fresh + p.per_tile - 1) / p.per_tile;
   }
   __device__ bool next() {
     if (t >= t_end) return false;
     if (started) {
       t0 = 0;
-      if (++qt >= tiles) {
+      if (++qt * p.per_tile >= fresh) {
         qt = 0;
         if (++h >= p.heads_kv) {
           h = 0;
@@ -151,15 +154,19 @@ struct PagedWalk {
 // front of a chunk's first unit, 3000 with this); the caller syncs behind it.
 struct PagedTables {
   int *cum, *len, *row;   // [batch + 1], [batch], [batch + 1] in shared memory
-  int* start;             // sequence, KV head, query tile and tile of that unit
-  static constexpr int kBytes = (3 * kPgMaxBatch + 6) * 4;
+  int* start;             // sequence, KV head, query tile and tile of that unit; the share [4], [5] in the list
+  static constexpr int kBytes = (3 * kPgMaxBatch + 8) * 4;
   __device__ explicit PagedTables(uint8_t* at)
       : cum(reinterpret_cast<int*>(at)), len(cum + kPgMaxBatch + 1), row(len + kPgMaxBatch), start(row + kPgMaxBatch + 1) {}
 
   __device__ void locate(const PagedParams& p) const {   // by a warp
     const int lane = threadIdx.x & 31, total = cum[p.batch], shares = min(static_cast<int>(gridDim.x), total);
-    if (static_cast<int>(blockIdx.x) >= shares) return;
-    const int t = pg_share(total, blockIdx.x, shares);
+    const int cta = static_cast<int>(blockIdx.x);
+    if (cta >= shares) {
+      if (lane == 0) start[4] = start[5] = 0;
+      return;
+    }
+    const int t = pg_share(total, cta, shares);
     int b = 0;   // last sequence with cum[b] <= t: it has tiles
     for (int i0 = 0; i0 < p.batch; i0 += 32) {
       const uint32_t in = __ballot_sync(0xffffffffu, i0 + lane < p.batch && cum[i0 + lane] <= t);
@@ -195,6 +202,8 @@ struct PagedTables {
       start[1] = h;
       start[2] = qt;
       start[3] = rest;
+      start[4] = t;
+      start[5] = pg_share(total, cta + 1, shares);
     }
   }
 
@@ -273,9 +282,8 @@ struct PagedShare {
   __device__ PagedShare(const PagedParams& p, const PagedTables& tab) {
     total = tab.cum[p.batch];
     shares = min(static_cast<int>(gridDim.x), total);   // none is empty
-    const int cta = blockIdx.x;
-    t0 = cta < shares ? pg_share(total, cta, shares) : 0;
-    t1 = cta < shares ? pg_share(total, cta + 1, shares) : 0;
+    t0 = tab.start[4];
+    t1 = tab.start[5];
   }
 };
 
