@@ -109,7 +109,7 @@ inline int plan_paged(const AttnB200PagedAttnArgs* a, int sms, PagedPlan* d) {
   long long unit_tiles = (most_kv + kPgTile - 1) / kPgTile;   // at most
   if (a->window > 0) unit_tiles = std::min<long long>(unit_tiles, (static_cast<long long>(a->window) + d->per_tile - 2) / kPgTile + 2);
   d->whole = unit_tiles <= kPgWholeTiles;
-  const long long most = q_tiles * c.heads_kv * (d->whole ? 1 : unit_tiles);
+  const long long most = q_tiles * c.heads_kv * (d->whole ? 1 : unit_tiles + kPgUnitCost);
   if (most > 0x3fffffff) return ATTN_B200_E_UNSUPPORTED;
   d->ctas = static_cast<int>(std::min<long long>(sms, most));
   const long long parts = d->whole ? 0 : 2LL * d->ctas * d->rows;

@@ -6,7 +6,7 @@
 // tiles of all units, in order, are cut into one equal share per SM: a long context against a single token is split over the
 // chip, the units of a prompt are spread over it evenly whatever their lengths, and a share walks its units with every ring
 // and barrier phase carried across them.  (Where no unit has more than four tiles, shares are whole units and there is nothing to
-// merge.)  A unit that lies in one share writes its rows; the others leave fp32 partial rows
+// merge; else a unit counts two tiles more than it has, for its beginning and end.)  A unit that lies in one share writes its rows; the others leave fp32 partial rows
 // that a second small kernel adds up (paged_attention.cu).  Each CTA counts the list itself from the lengths on the device,
 // so a captured call follows them.
 // Pages are fetched by TMA, a box of up to 128 rows of one page, its index from the block table; boxes without a row that
@@ -28,6 +28,10 @@ namespace b200 {
 
 constexpr int kPgTile = 128;       // KV rows of a tile
 constexpr int kPgMaxBatch = 1024;  // sequences of a call
+
+// What a unit's beginning and end cost, in tiles, where the list is cut into equal shares: 16 batches of chunks and tokens of
+// all kinds took 55 us in the mean with 0, 50 with 1, 48 with 2, 48.5 with 4.
+constexpr int kPgUnitCost = 2;
 
 struct PagedParams {
   void* o;
@@ -101,9 +105,10 @@ struct PagedSpan {
 struct PagedWalk {
   const PagedParams& p;
   const int *cum, *lens, *row0;
-  int t, t_end;                      // the share, in tiles of the list (whole: in units)
+  int t, t_end;                      // the share, in tiles of the list, kPgUnitCost of them in front of every unit's own (whole: in units)
   int b, h, qt, len, fresh;          // sequence, KV head, query tile; its length, new tokens
-  int begin, end, lo, total, t0, n;  // keys and KV tiles of the unit; this share's: n from t0 on
+  int begin, end, lo, total, t0, n;  // keys and KV tiles of the unit; this share's: n from t0 on (before the first next(): the place in the unit)
+  int last;                          // place of the unit's last tile in the list
   bool started = false;
   __device__ PagedWalk(const PagedParams& p_, const int* cum_, const int* lens_, const int* row0_, const int* start, int t_, int t_end_)
       : p(p_), cum(cum_), lens(lens_), row0(row0_), t(t_), t_end(t_end_) {
@@ -137,9 +142,17 @@ struct PagedWalk {
     end = s.end;
     lo = s.lo;
     total = s.n;
-    n = p.whole ? total : min(total - t0, t_end - t);
-    t += p.whole ? 1 : n;
-    return true;
+    if (p.whole) {
+      n = total;
+      ++t;
+      return true;
+    }
+    const int to = min(total + kPgUnitCost, t0 + t_end - t);
+    last = t - t0 + total + kPgUnitCost - 1;
+    t += to - t0;
+    t0 = max(t0 - kPgUnitCost, 0);
+    n = max(to - kPgUnitCost, 0) - t0;
+    return n > 0;   // 0: the share ends in front of the unit's tiles
   }
   // rows [a, e) of the unit's i-th tile that any of its rows sees
   __device__ void rows_of(int i, int& a, int& e) const {
@@ -180,7 +193,7 @@ struct PagedTables {
     } else {
       const int fresh = row[b + 1] - row[b], tiles = (fresh + p.per_tile - 1) / p.per_tile;
       for (int q0 = 0; q0 < tiles; q0 += 32) {
-        const int n = q0 + lane < tiles ? PagedSpan(p, len[b], fresh, q0 + lane).n : 0;
+        const int n = q0 + lane < tiles ? PagedSpan(p, len[b], fresh, q0 + lane).n + kPgUnitCost : 0;
         int x = n;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -240,14 +253,14 @@ struct PagedTables {
     if (p.cu == nullptr && p.seq <= 4 * p.per_tile) {   // a few query tiles: a thread a sequence
       for (int b = tid; b < p.batch; b += threads) {
         int sum = 0;
-        for (int qt = 0; qt * p.per_tile < p.seq; ++qt) sum += p.whole ? 1 : PagedSpan(p, len[b], p.seq, qt).n;
+        for (int qt = 0; qt * p.per_tile < p.seq; ++qt) sum += p.whole ? 1 : PagedSpan(p, len[b], p.seq, qt).n + kPgUnitCost;
         cum[b] = sum * p.heads_kv;
       }
     } else {
       for (int b = warp; b < p.batch; b += threads / 32) {
         const int fresh = row[b + 1] - row[b], tiles = (fresh + p.per_tile - 1) / p.per_tile;
         int sum = 0;
-        for (int qt = lane; qt < tiles; qt += 32) sum += p.whole ? 1 : PagedSpan(p, len[b], fresh, qt).n;
+        for (int qt = lane; qt < tiles; qt += 32) sum += p.whole ? 1 : PagedSpan(p, len[b], fresh, qt).n + kPgUnitCost;
         if (tiles > 1) {
 #pragma unroll
           for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);

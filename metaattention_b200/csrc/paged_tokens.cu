@@ -461,8 +461,8 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
           else if (p.lse != nullptr) p.lse[(p.cu != nullptr ? static_cast<long long>(head) : static_cast<long long>(u.b) * p.heads + head) * p.seq + row0 + tok] = lse;
         }
       }
-      if (tid == 0 && !whole && u.t0 == 0)   // t is behind the unit's part
-        p.cut[cta] = make_int4(u.b, u.h, u.qt, pg_owner(u.t - u.n + u.total - 1, share.shares, share.total));
+      if (tid == 0 && !whole && u.t0 == 0)
+        p.cut[cta] = make_int4(u.b, u.h, u.qt, pg_owner(u.last, share.shares, share.total));
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(bars + L::kOFree + (ui & 1));
