@@ -212,7 +212,7 @@ int paged_setup(const AttnB200PagedAttnArgs* a, const PagedPlan& d, int* status,
   while ((1 << p.page_shift) < c.page_size) ++p.page_shift;
   while ((1 << p.box_shift) < box) ++p.box_shift;
   p.causal = a->causal != 0;
-  p.window = a->window;
+  p.window = std::min(a->window, 0x3fffffff);   // no sequence is longer, and a position less it stays in 32 bits
   p.whole = d.whole ? 1 : 0;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   p.part_o = reinterpret_cast<float*>(ws);

@@ -708,3 +708,28 @@ def test_memory_that_a_call_must_not_write_is_refused():
         RotaryEmbedding(64)(q, q, inplace=True)
     own = q.clone()
     assert torch.equal(c.cache.attention(own, t, s, out=own), c.cache.attention(q, t, s))   # in q's place
+
+
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("news", [[1, 1, 1, 1], [1, 40, 3, 7]])
+def test_padding_rows_may_hold_anything(codes, news):
+    """Rows of q behind the last sequence that are NaN or infinite touch no row of a sequence, in the tile they share with its last ones."""
+    lens, H, D, pad = [30, 300, 129, 64], 8, 64, 5
+    c = Case(lens, 2, D, 16, torch.float16, codes, seed=93)
+    q, qd, cu = fresh_rows(news, (H, D), torch.float16, True, 94, pad)
+    qd[sum(news):sum(news) + 3] = float("nan")
+    qd[sum(news) + 3:] = float("inf")
+    o, lse = c.cache.attention(qd, c.block_table, c.cache_seqlens, cu_seqlens=cu, return_lse=True)
+    check_attention(c, news, q[:sum(news)], o[:sum(news)], lse, True, H)
+
+
+def test_windows_of_any_size():
+    """A window as long as numbers go is none, chunks and single tokens, more new tokens than tokens among them."""
+    for news in ([9, 9], [1, 1]):
+        c = Case([5, 300], 1, 64, 16, torch.bfloat16, False, seed=95)
+        q, qd, _ = fresh_rows(news, (4, 64), torch.bfloat16, False, 96)
+        plain = c.cache.attention(qd, c.block_table, c.cache_seqlens, return_lse=True)
+        for window in (301, 1 << 29, 2 ** 31 - 1, 2 ** 40):
+            wide = c.cache.attention(qd, c.block_table, c.cache_seqlens, window=window, return_lse=True)
+            check_attention(c, news, q, *wide, False, 4)
+            assert torch.equal(wide[1] == -math.inf, plain[1] == -math.inf)

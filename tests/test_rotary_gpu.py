@@ -224,3 +224,30 @@ def test_other_stream_and_captured_replay():
     with pytest.raises(lib.NativeError):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             fresh(buf)
+
+
+def test_captured_training_step():
+    """Forward and backward in one graph, replayed with other inputs, positions and gradients."""
+    rope = RotaryEmbedding(64)
+    q, k = (draw((2, 33, h, 64), torch.bfloat16, 30 + h).cuda().requires_grad_() for h in (4, 2))
+    gq, gk = (draw((2, 33, h, 64), torch.bfloat16, 40 + h).cuda() for h in (4, 2))
+    pos = torch.arange(33).cuda()
+
+    def step():
+        yq, yk = rope(q, k, pos)
+        return (yq.detach(), yk.detach(), *torch.autograd.grad((yq, yk), (q, k), (gq, gk)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for seed in (50, 60):
+        with torch.no_grad():
+            for i, t in enumerate((q, k, gq, gk)):
+                t.copy_(draw(tuple(t.shape), torch.bfloat16, seed + i).cuda())
+            pos.add_(777)
+        g.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))
