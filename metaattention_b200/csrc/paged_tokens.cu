@@ -16,7 +16,8 @@
 // Measured: 64 sequences of up to 8192 tokens, 32 heads on 8 KV heads of 128: 206 us, 6.5 TB/s of the cache's bytes, the rate of a
 // copy.  8 bits, 16 sequences of up to 32768: 173 us, 4.3 TB/s: per tile of 128 rows (1130 ns) the widening of V and the softmax take
 // turns at the issue slots of twenty warps; a single sequence of 333 tokens 8.2 us, start, two tiles and end.
-// Units of 17 to 32 rows in 8 bits spill (640 bytes a thread, 32 rows of scores and sums in 96 registers).
+// Units of 17 to 32 rows in 8 bits (32 rows of scores and sums in 96 registers): 16 sequences of 16384 tokens 164 us with 20 rows, 218 with
+// 32, where 16 rows take 141, and the same in 16 bits 168.
 #include <cstring>
 
 #include "paged_common.cuh"
@@ -339,15 +340,23 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
             s[r] = in ? s[r] : -INFINITY;
           }
         }
-        float ref[R], over = -INFINITY;
+        // 16 rows in 8 bits hold their reference maxima and rescales (173 us for 182, 16 sequences of up to 32768); else they are read
+        // again where they are used: 32 rows in 8 bits spilled with them (298 us for 218, 16 sequences of 16384, 32 rows)
+        constexpr bool kHold = k8Bit && R == 16;
+        float ref[kHold ? R : 1], over = -INFINITY;
+        auto hold = [&](int r, const float4& m) {
+          if constexpr (kHold) {
+            ref[r] = m.x;
+            ref[r + 1] = m.y;
+            ref[r + 2] = m.z;
+            ref[r + 3] = m.w;
+          }
+        };
 #pragma unroll
         for (int r = 0; r < R; r += 4) {
           if (r >= p.rows) break;
           const float4 m = reinterpret_cast<const float4*>(s_ref)[r / 4];
-          ref[r] = m.x;
-          ref[r + 1] = m.y;
-          ref[r + 2] = m.z;
-          ref[r + 3] = m.w;
+          hold(r, m);
           over = max3(over, s[r] - m.x, s[r + 1] - m.y);
           over = max3(over, s[r + 2] - m.z, s[r + 3] - m.w);
         }
@@ -369,18 +378,27 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
             if (grown) s_ref[key0] = m;
           }
           sync();
-          float scale[R];
+          float scale[kHold ? R : 1];
 #pragma unroll
           for (int r = 0; r < R; r += 4) {
             if (r >= p.rows) break;
-            const float4 m = reinterpret_cast<const float4*>(s_ref)[r / 4], x = reinterpret_cast<const float4*>(s_rescale)[r / 4];
-            ref[r] = m.x; ref[r + 1] = m.y; ref[r + 2] = m.z; ref[r + 3] = m.w;
-            scale[r] = x.x; scale[r + 1] = x.y; scale[r + 2] = x.z; scale[r + 3] = x.w;
+            const float4 x = reinterpret_cast<const float4*>(s_rescale)[r / 4];
+            if constexpr (kHold) {
+              hold(r, reinterpret_cast<const float4*>(s_ref)[r / 4]);
+              scale[r] = x.x; scale[r + 1] = x.y; scale[r + 2] = x.z; scale[r + 3] = x.w;
+            } else {
+              acc[r] *= x.x;
+              acc[r + 1] *= x.y;
+              acc[r + 2] *= x.z;
+              acc[r + 3] *= x.w;
+            }
           }
+          if constexpr (kHold) {
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            if (r % 4 == 0 && r >= p.rows) break;
-            acc[r] *= scale[r];
+            for (int r = 0; r < R; ++r) {
+              if (r % 4 == 0 && r >= p.rows) break;
+              acc[r] *= scale[r];
+            }
           }
           if (i >= 2) {   // behind the group's last P.V
             mbar_wait_rows(bars + L::kODone + group, ((J >> 1) - 1) & 1, ab, kPgODone);
@@ -391,7 +409,7 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
               tmem_ld16f(tOg + c, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int r = 0; r < 16; ++r) o[r] *= scale[c + r];
+              for (int r = 0; r < 16; ++r) o[r] *= kHold ? scale[kHold ? c + r : 0] : s_rescale[c + r];
               tmem_st16f(tOg + c, o);
             }
             tmem_wait_st();
@@ -399,10 +417,14 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
         }
         // the operand's buffer is free behind the group's last P.V
         if (J >= 2) mbar_wait_rows(bars + L::kODone + group, ((J >> 1) - 1) & 1, ab, kPgODone);
+        float4 m;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          if (r % 4 == 0 && r >= p.rows) break;   // four rows at a time, those that there are
-          const float x = fast_exp2(s[r] - ref[r]);
+          if (r % 4 == 0) {   // four rows at a time, those that there are
+            if (r >= p.rows) break;
+            if (!kHold) m = reinterpret_cast<const float4*>(s_ref)[r / 4];
+          }
+          const float x = fast_exp2(s[r] - (kHold ? ref[kHold ? r : 0] : r % 4 == 0 ? m.x : r % 4 == 1 ? m.y : r % 4 == 2 ? m.z : m.w));
           acc[r] += x;
           const uint32_t two = pack2<kBf16>(x, 0.0f);
           asm volatile("st.shared.u16 [%0], %1;" ::"r"(line + r * 128 + ((p_piece ^ (r & 7)) << 4)), "h"(static_cast<uint16_t>(two)) : "memory");
