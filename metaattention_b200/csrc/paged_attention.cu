@@ -95,8 +95,10 @@ inline int plan_paged(const AttnB200PagedAttnArgs* a, int sms, PagedPlan* d) {
   const bool packed = a->cu_seqlens != nullptr;
   const long long all = packed ? a->seq : static_cast<long long>(c.batch) * a->seq;   // new tokens
   if (all > 0x7fffffff / 2) return ATTN_B200_E_UNSUPPORTED;
-  // A few rows a sequence: their own kernel.  How many a packed sequence has the host does not know; where they are less than
-  // two on average a longer one among them costs a walk over its keys for each kPgFew of its rows.
+  // A few rows a sequence: their own kernel (16 sequences of 16384, 20 rows: 168 us where paged_chunk.cu takes 183, 64 columns 97 for
+  // 177, 8 bits 165 for 281).  How many a packed sequence has the host does not know; where they are less than two on average a
+  // longer one among them costs a walk over its keys for each kPgFew of its rows (64 sequences of up to 8192, single tokens: 208 us
+  // for 230, 8 bits 212 for 352; 63 and one of 60 tokens: 229 for 291, 274 for 469).
   d->few = d->group <= kPgFew && (packed ? a->seq < 2LL * c.batch : static_cast<long long>(d->group) * a->seq <= kPgFew);
   // packed tokens, most of them alone: the narrower score tile
   const int most_rows = !d->few ? kPgTile : packed && d->group <= kPgFew / 2 ? kPgFew / 2 : kPgFew;
