@@ -8,6 +8,7 @@ lse: 2^-17 (1 + |lse|)."""
 
 import ctypes
 import math
+import random
 
 import pytest
 import torch
@@ -733,3 +734,22 @@ def test_windows_of_any_size():
             wide = c.cache.attention(qd, c.block_table, c.cache_seqlens, window=window, return_lse=True)
             check_attention(c, news, q, *wide, False, 4)
             assert torch.equal(wide[1] == -math.inf, plain[1] == -math.inf)
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_random_calls(seed):
+    """Batches of any kind: lengths, new tokens, heads, pages, windows, layouts and types drawn together."""
+    r = random.Random(seed)
+    B, Hkv, D, page = r.choice([1, 2, 5, 17, 40]), r.choice([1, 2, 3, 8]), r.choice([64, 128]), r.choice([8, 16, 64, 128, 512])
+    H = Hkv * r.choice([1, 2, 3, 4, 7, 8, 20])
+    lens = [r.choice([0, 1, 127, 128, 129, r.randint(1, 700), r.randint(1, 2500)]) for _ in range(B)]
+    packed, kind = r.random() < 0.6, r.choice(["one", "few", "many"])
+    most = {"one": 1, "few": 6, "many": 90}[kind]
+    n = r.randint(1, most)
+    news = [r.choice([0, 1, 1, r.randint(1, most)]) for _ in range(B)] if packed else [n] * B
+    if sum(news) == 0:
+        news[0] = 1
+    causal = r.random() < 0.85
+    window = r.choice([None, None, 1, 63, 500, 1500]) if causal else None
+    run_attention(lens, news, H, Hkv, D, page, r.choice([torch.bfloat16, torch.float16]), r.random() < 0.5, packed=packed, seed=seed, hnd=r.random() < 0.7,
+                  pad=r.choice([0, 0, 3, 200]) if packed else 0, causal=causal, window=window)
