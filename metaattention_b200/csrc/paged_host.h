@@ -58,7 +58,7 @@ std::vector<Tensor> rotary_launch(const Turns& turns, const std::vector<Tensor>&
   const Tensor& q = x[0];
   const int lead = q.dim() - 2;   // 1 or 2 axes of tokens
   for (const Tensor& t : x) y.push_back(inplace ? t : fresh(t.sizes(), t.scalar_type(), t));
-  if (q.numel() == 0) return y;
+  if (q.size(0) == 0 || q.size(lead - 1) == 0) return y;   // no tokens; q, or k, without heads is passed over below
   a.batch = lead == 2 ? q.size(0) : 1;
   a.seq = q.size(lead - 1);
   a.head_dim = q.size(-1);
