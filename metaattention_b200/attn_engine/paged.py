@@ -88,7 +88,7 @@ class PagedKVCache:
         negative position, gives 0 and -inf.  ``scale`` defaults to head_dim ** -0.5.  Written to ``out`` if given; packed rows
         behind the last sequence are left as they are there (and are not initialised otherwise).  An 8-bit cache is read as
         the values of q's dtype that its codes stand for.  Keys and values inside a sequence must be finite; what lies behind
-        its end is not looked at.  No backward pass."""
+        its end is not looked at.  No backward pass, and no forward-mode one."""
         if window is not None and window <= 0:
             raise ValueError(f"window must be positive (got {window})")
         o, lse = native.host().cache_attention(self._native, q, block_table, cache_seqlens, cu_seqlens,

@@ -105,7 +105,8 @@ class RotaryEmbedding:
         """q: [batch, seq, heads, head_dim] or packed [tokens, heads, head_dim], k the same with heads of its own; float16,
         bfloat16 or float32, any strides with a contiguous last dimension.  ``positions``: int32 or int64 [batch, seq] or
         [seq] (packed: [tokens]), default 0, 1, ... along seq; negative ones turn backwards.  Computed in 32 bits and rounded
-        once.  Differentiable in q and k (twice too); ``inplace`` writes over q and k instead and keeps no graph.
+        once.  Differentiable in q and k (twice too; tangents of forward mode are refused); ``inplace`` writes over q and k
+        instead and keeps no graph.
         In a captured training step, as with every operation of torch, no graph made outside of the capture may still hold the leaves."""
         if not q.is_cuda:
             raise native.NativeError("rotary positions need CUDA tensors: there is no CPU path")

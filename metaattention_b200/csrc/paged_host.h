@@ -32,6 +32,13 @@ bool wide_strides(const Tensor& t, int64_t unit) {   // whole 16-byte pieces
   return t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
+// A tangent of forward mode beside the values: these launches would leave it behind without a word.
+void no_tangent(const char* what, std::initializer_list<const Tensor*> given) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : given)
+    if (t->defined() && t->_fw_grad(0).defined()) refuse(what, " has no forward-mode derivative (torch.autograd.forward_ad): a tensor of the call carries a tangent");
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 // rotary positions
 // ---------------------------------------------------------------------------------------------------------------
@@ -148,8 +155,10 @@ std::vector<Tensor> rotary_call(const std::shared_ptr<const Turns>& turns, const
     if (k->scalar_type() != type || k->device() != q.device()) refuse("q and k must share dtype and device");
     x.push_back(*k);
   }
-  for (const Tensor& t : x)
+  for (const Tensor& t : x) {
+    no_tangent("a rotation by positions", {&t});
     if (t.numel() > 0 && t.stride(-1) != 1) refuse("the last dimension must be contiguous");
+  }
   if (positions.has_value()) {
     const Tensor& p = *positions;
     if (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong) refuse("positions must be int32 or int64 (got ", p.scalar_type(), ")");
@@ -288,6 +297,7 @@ void cache_append(const Cache& c, const Tensor& k, const Tensor& v, const Tensor
   AttnB200PagedAppendArgs a;
   std::memset(&a, 0, sizeof(a));
   Tensor held;
+  no_tangent("a cache", {&k, &v, &c.k, &c.v});
   a.cache = sequences(c, table, lens, held);
   new_rows(c, k, "k", cu, a.cache.batch, a.cache.heads_kv);
   new_rows(c, v, "v", cu, a.cache.batch, a.cache.heads_kv);
@@ -317,6 +327,7 @@ std::vector<Tensor> cache_read(const Cache& c, const Tensor& table, const Tensor
   AttnB200PagedReadArgs a;
   std::memset(&a, 0, sizeof(a));
   Tensor held;
+  no_tangent("a cache", {&c.k, &c.v});
   a.cache = sequences(c, table, lens, held);
   if (max_len < 0 || max_len > 0x7fffffff) refuse("max_len must not be negative (got ", max_len, ")");
   if (at::GradMode::is_enabled() && (c.k.requires_grad() || c.v.requires_grad())) refuse("a cache has no gradient: read it under torch.no_grad()");
@@ -341,6 +352,8 @@ std::tuple<Tensor, OptTensor> cache_attention(const Cache& c, const Tensor& q, c
   AttnB200PagedAttnArgs a;
   std::memset(&a, 0, sizeof(a));
   Tensor held;
+  no_tangent("attention over a paged cache", {&q, &c.k, &c.v});
+  if (out.has_value()) no_tangent("attention over a paged cache", {&*out});
   a.cache = sequences(c, table, lens, held);
   if (q.dim() < 3) refuse("q must be [batch, seq, heads, head_dim], or [rows, heads, head_dim] with cu_seqlens, got ", shape_of(q));
   const int64_t H = q.size(-2), Hkv = a.cache.heads_kv;

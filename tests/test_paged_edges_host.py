@@ -1,0 +1,40 @@
+"""What calls of rotary positions and of paged caches are refused for, without a GPU: the host side looks at the tensors before
+anything is launched, so tensors of the CPU do."""
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from attn_engine import PagedKVCache
+from core.native import lib
+
+
+def pools(pages=4, page=16, heads=2, D=64, dtype=torch.bfloat16):
+    return torch.zeros(pages, page, heads, D, dtype=dtype), torch.zeros(pages, page, heads, D, dtype=dtype)
+
+
+def rotary(*args):
+    """The native call behind RotaryEmbedding, with frequencies on the CPU."""
+    host = lib.host()
+    return host.rotary(host.make_turns(torch.zeros(32, dtype=torch.int64), 64, False, 1.0), *args)
+
+
+def test_tangents_of_forward_mode_are_refused():
+    """A dual tensor whose primal wants no gradient would come back without its tangent."""
+    x, plain = torch.ones(2, 1, 2, 64), torch.ones(2, 1, 2, 64, dtype=torch.bfloat16)
+    cache, table, lens = PagedKVCache(*pools()), torch.zeros(2, 2, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    with forward_ad.dual_level():
+        dual, dual16 = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(plain, torch.ones_like(plain))
+        held = PagedKVCache(*(forward_ad.make_dual(t, torch.ones_like(t)) for t in pools()))
+        calls = [lambda: rotary(dual, None, None, False), lambda: rotary(x, dual, None, False), lambda: rotary(dual, None, None, True),
+                 lambda: rotary(dual[:, :, :1], None, None, False),   # a view of one
+                 lambda: cache.attention(dual16, table, lens), lambda: cache.attention(plain, table, lens, out=dual16),
+                 lambda: cache.append(dual16, plain, table, lens), lambda: cache.append(plain, dual16, table, lens),
+                 lambda: held.attention(plain, table, lens), lambda: held.append(plain, plain, table, lens), lambda: held.read(table, lens, 4)]
+        for call in calls:
+            with pytest.raises(ValueError, match="forward"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="forward"):   # which does not turn forward mode off
+                call()
+        with forward_ad._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="CUDA"):   # the next refusal
+            cache.attention(dual16, table, lens)
