@@ -58,7 +58,8 @@ class RotaryEmbedding:
     ``interleaved``: pairs of neighbouring columns (2 i, 2 i + 1) instead of (i, i + rotary_dim / 2); columns from
     ``rotary_dim`` on stay as they are.  The frequencies are those of ``rotary_frequencies``, or ``frequencies``
     (``rotary_dim / 2`` values in radians per position) with ``magnitude``.  The first call on a device lays them out there:
-    make it before capturing a CUDA graph."""
+    make it before capturing a CUDA graph.  Calls on any stream and captured graphs keep what they read, also when the
+    RotaryEmbedding itself is gone."""
 
     def __init__(self, rotary_dim: int, base: float = 10000.0, interleaved: bool = False, scaling: str | None = None, factor: float = 1.0,
                  original_length: int = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0, frequencies=None, magnitude: float | None = None):

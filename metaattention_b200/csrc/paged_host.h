@@ -55,6 +55,33 @@ struct Turns {   // what a RotaryEmbedding decided at construction, on one devic
     r.interleaved = interleaved;
     r.magnitude = magnitude;
   }
+
+  // Around a launch on the current stream: the RotaryEmbedding may go with that launch still to run, and the memory must then not
+  // be handed out again before it has.  Told to the allocator once for each stream.  A captured launch reads the table whenever
+  // its graph is replayed, which nobody announces: that table stays for good.
+  void used() const {
+    const auto now = c10::cuda::getCurrentCUDAStream(turns.device().index());
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (kept_) return;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    C10_CUDA_CHECK(cudaStreamIsCapturing(now.stream(), &capture));
+    if (capture != cudaStreamCaptureStatusNone) {
+      static auto* kept = new std::vector<Tensor>();
+      static std::mutex kept_mutex;
+      std::lock_guard<std::mutex> all(kept_mutex);
+      kept->push_back(turns);
+      kept_ = true;
+      return;
+    }
+    if (std::find(streams_.begin(), streams_.end(), now.stream()) != streams_.end()) return;
+    c10::cuda::CUDACachingAllocator::recordStream(turns.storage().data_ptr(), now);
+    streams_.push_back(now.stream());
+  }
+
+ private:
+  mutable std::mutex mutex_;
+  mutable std::vector<cudaStream_t> streams_;
+  mutable bool kept_ = false;
 };
 
 // y = x turned, for x = q and perhaps k; [tokens, heads, D] or [batch, seq, heads, D]
@@ -72,6 +99,7 @@ std::vector<Tensor> rotary_launch(const Turns& turns, const std::vector<Tensor>&
   a.dtype = q.scalar_type() == at::kFloat ? ATTN_B200_DTYPE_FP32 : dtype_code(q);
   a.inverse = inverse;
   turns.fill(a.rotary);
+  turns.used();
   int n = 0;
   for (size_t i = 0; i < x.size(); ++i) {
     if (x[i].size(lead) == 0) continue;   // no heads
@@ -318,6 +346,7 @@ void cache_append(const Cache& c, const Tensor& k, const Tensor& v, const Tensor
   a.dtype = dtype_code(k);
   py::gil_scoped_release others_run;
   c10::cuda::CUDAGuard guard(k.device());
+  if (turns != nullptr) turns->used();
   check(paged_api.append(&a, stream_of(k)), "attn_b200_paged_append");
   for (const Tensor* t : {&c.k, &c.v, &c.k_scale, &c.v_scale})
     if (t->defined() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();   // a graph that has saved it finds out

@@ -2,10 +2,12 @@
 asked for, frequencies that leave while they are read, batches whose first rows go backwards, broadcast queries, pools that moved.
 Tolerances are those of test_rotary_gpu.py and test_paged_gpu.py."""
 
+import gc
+
 import pytest
 import torch
 
-from attn_engine import RotaryEmbedding
+from attn_engine import PagedKVCache, RotaryEmbedding
 from core.native import lib
 
 pytestmark = pytest.mark.gpu
@@ -40,3 +42,44 @@ def test_queries_without_heads_leave_the_keys_their_rotation(packed, dtype):
     dq, dk = torch.autograd.grad((a, b), (empty, leaf), (torch.empty_like(a), g))
     assert dq.shape == q.shape and torch.equal(dk, alone)
     assert lib.last_device_status() == 0
+
+
+def overwrite_what_is_free():
+    """Blocks of the size of a small table, from the current stream's memory, with other contents."""
+    return [torch.full((n,), -(2 ** 61) + 12345, dtype=torch.int64, device="cuda") for n in (32, 64) for _ in range(200)]
+
+
+def test_frequencies_outlive_their_embedding_on_other_streams():
+    """First call on one stream, another behind a long kernel on a second one, the embedding gone, new memory on the first."""
+    x = draw((40, 4, 64), torch.bfloat16, 3).cuda()
+    want = RotaryEmbedding(64, base=777.0)(x)
+    gc.collect()
+    torch.cuda.synchronize()
+    rope, side = RotaryEmbedding(64, base=777.0), torch.cuda.Stream()
+    rope(x)
+    cache = PagedKVCache.allocate(4, 16, 4, 64)
+    table, lens = torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4), torch.tensor([40], dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)   # a tenth of a second
+        got = rope(x)
+        cache.append(x.unsqueeze(0), x.unsqueeze(0), table, lens, rotary=rope)
+    del rope
+    gc.collect()
+    other = overwrite_what_is_free()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(cache.read(table, lens, 40)[0][0], want) and len(other) == 400
+
+
+def test_frequencies_outlive_their_embedding_in_a_graph():
+    x = draw((40, 4, 64), torch.bfloat16, 4).cuda()
+    rope, g = RotaryEmbedding(64, base=555.0), torch.cuda.CUDAGraph()
+    want = rope(x)
+    with torch.cuda.graph(g):
+        got = rope(x)
+    del rope
+    gc.collect()
+    other = overwrite_what_is_free()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and len(other) == 400
