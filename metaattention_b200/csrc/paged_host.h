@@ -34,9 +34,9 @@ bool wide_strides(const Tensor& t, int64_t unit) {   // whole 16-byte pieces
 
 // A tangent of forward mode beside the values: these launches would leave it behind without a word.
 void no_tangent(const char* what, std::initializer_list<const Tensor*> given) {
-  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
   for (const Tensor* t : given)
-    if (t->defined() && t->_fw_grad(0).defined()) refuse(what, " has no forward-mode derivative (torch.autograd.forward_ad): a tensor of the call carries a tangent");
+    if (t->_fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+      refuse(what, " has no forward-mode derivative (torch.autograd.forward_ad): a tensor of the call carries a tangent");
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -61,10 +61,11 @@ struct Turns {   // what a RotaryEmbedding decided at construction, on one devic
   // its graph is replayed, which nobody announces: that table stays for good.
   void used() const {
     const auto now = c10::cuda::getCurrentCUDAStream(turns.device().index());
-    std::lock_guard<std::mutex> lock(mutex_);
-    if (kept_) return;
+    if (kept_.load(std::memory_order_relaxed)) return;
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     C10_CUDA_CHECK(cudaStreamIsCapturing(now.stream(), &capture));
+    if (capture == cudaStreamCaptureStatusNone && told_.load(std::memory_order_relaxed) == now.id()) return;   // as the last call
+    std::lock_guard<std::mutex> lock(mutex_);
     if (capture != cudaStreamCaptureStatusNone) {
       static auto* kept = new std::vector<Tensor>();
       static std::mutex kept_mutex;
@@ -73,15 +74,18 @@ struct Turns {   // what a RotaryEmbedding decided at construction, on one devic
       kept_ = true;
       return;
     }
-    if (std::find(streams_.begin(), streams_.end(), now.stream()) != streams_.end()) return;
-    c10::cuda::CUDACachingAllocator::recordStream(turns.storage().data_ptr(), now);
-    streams_.push_back(now.stream());
+    if (std::find(streams_.begin(), streams_.end(), now.id()) == streams_.end()) {
+      c10::cuda::CUDACachingAllocator::recordStream(turns.storage().data_ptr(), now);
+      streams_.push_back(now.id());
+    }
+    told_ = now.id();
   }
 
  private:
   mutable std::mutex mutex_;
-  mutable std::vector<cudaStream_t> streams_;
-  mutable bool kept_ = false;
+  mutable std::vector<c10::StreamId> streams_;
+  mutable std::atomic<c10::StreamId> told_{std::numeric_limits<c10::StreamId>::min()};
+  mutable std::atomic<bool> kept_{false};
 };
 
 // y = x turned, for x = q and perhaps k; [tokens, heads, D] or [batch, seq, heads, D]
