@@ -137,7 +137,7 @@ struct TurnsRef : torch::CustomClassHolder {
 };
 
 // The map is linear and its transpose is the map by the opposite angles, so the backward is the same function again, and
-// differentiable itself.
+// differentiable itself.  Only what asks for a gradient gets one, on both ways.
 struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const std::shared_ptr<const Turns>& turns, bool inverse,
                                                 const OptTensor& positions, const Tensor& q, const OptTensor& k) {
@@ -150,7 +150,12 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     at::AutoDispatchBelowADInplaceOrView below;
     std::vector<Tensor> x{q};
     if (k.has_value()) x.push_back(*k);
-    return rotary_launch(*turns, x, positions, inverse, false);
+    auto y = rotary_launch(*turns, x, positions, inverse, false);
+    std::vector<Tensor> constant;
+    for (size_t i = 0; i < x.size(); ++i)
+      if (!x[i].requires_grad()) constant.push_back(y[i]);
+    ctx->mark_non_differentiable(constant);
+    return y;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto ref = c10::static_intrusive_pointer_cast<TurnsRef>(ctx->saved_data["turns"].toCapsule());
@@ -160,7 +165,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     std::vector<int> which;
     std::vector<Tensor> g;
     for (size_t i = 0; i < grads.size(); ++i)
-      if (grads[i].defined()) {
+      if (grads[i].defined() && ctx->needs_input_grad((saved.defined() ? 1 : 0) + i)) {   // counted over the tensors of the call
         which.push_back(static_cast<int>(i));
         g.push_back(grads[i].stride(-1) == 1 || grads[i].numel() == 0 ? grads[i] : grads[i].contiguous());
       }

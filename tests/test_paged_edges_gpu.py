@@ -44,6 +44,34 @@ def test_queries_without_heads_leave_the_keys_their_rotation(packed, dtype):
     assert lib.last_device_status() == 0
 
 
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("both", [False, True])
+def test_only_what_asks_for_a_gradient_gets_one(given, both):
+    """An operand that wants none comes back without a graph (and may be appended); of two, each gradient is had by itself."""
+    rope = RotaryEmbedding(64)
+    pos = torch.arange(5, device="cuda") + 90 if given else None
+    x, gx = draw((2, 5, 4, 64), torch.bfloat16, 5).cuda(), draw((2, 5, 4, 64), torch.bfloat16, 6).cuda()
+    y, gy = draw((2, 5, 2, 64), torch.bfloat16, 7).cuda(), draw((2, 5, 2, 64), torch.bfloat16, 8).cuda()
+    alone = []
+    for t, g in ((x, gx), (y, gy)):
+        leaf = t.clone().requires_grad_()
+        alone += torch.autograd.grad(rope(leaf, positions=pos), leaf, g)
+    for which in (0, 1):
+        q, k = x.clone().requires_grad_(both or which == 0), y.clone().requires_grad_(both or which == 1)
+        a, b = rope(q, k, positions=pos)
+        assert a.requires_grad == q.requires_grad and b.requires_grad == k.requires_grad
+        outputs, grads = ((a, b), (gx, gy)) if both else ((a, b)[which], (gx, gy)[which])
+        (d,) = torch.autograd.grad(outputs, (q, k)[which], grads, retain_graph=True)
+        assert torch.equal(d, alone[which])
+        (again,) = torch.autograd.grad((a, b)[which], (q, k)[which], (gx, gy)[which], create_graph=True)
+        assert torch.equal(again, alone[which])
+        if not both and which == 0:
+            cache = PagedKVCache.allocate(2, 16, 2, 64)
+            table, lens = torch.tensor([[0], [1]], dtype=torch.int32, device="cuda"), torch.tensor([5, 5], dtype=torch.int32, device="cuda")
+            cache.append(b, b, table, lens)
+            assert torch.equal(cache.read(table, lens, 5)[0], b)
+
+
 def overwrite_what_is_free():
     """Blocks of the size of a small table, from the current stream's memory, with other contents."""
     return [torch.full((n,), -(2 ** 61) + 12345, dtype=torch.int64, device="cuda") for n in (32, 64) for _ in range(200)]
