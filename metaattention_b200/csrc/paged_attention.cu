@@ -20,11 +20,9 @@ __global__ void __launch_bounds__(2 * D) paged_merge_kernel(const __grid_constan
   const int4 cut = __ldcg(p.cut + c_lo);
   if (cut.w < 0 || row >= p.rows || r >= p.tile_pos * p.group) return;
   const int tok = cut.z * p.per_tile + t * p.tile_pos + qi, head = cut.y * p.group + g;
-  int row0 = 0, fresh = p.seq;
-  if (p.cu != nullptr) {
-    row0 = min(max(p.cu[cut.x], 0), p.seq);
-    fresh = min(max(p.cu[cut.x + 1], 0), p.seq) - row0;
-  }
+  // rows as the kernel in front of this one counted them: those of p.cu may go backwards
+  const int2 seq_rows = __ldcg(p.cut_rows + c_lo);
+  const int row0 = seq_rows.x, fresh = seq_rows.y;
   if (tok >= fresh) return;
   const int c_hi = min(cut.w, ctas - 1);
   float mx = -INFINITY, den = 0.0f, acc[8];
@@ -117,7 +115,8 @@ inline int plan_paged(const AttnB200PagedAttnArgs* a, int sms, PagedPlan* d) {
   const long long parts = d->whole ? 0 : 2LL * d->ctas * d->rows;
   d->off_lse = parts * c.head_dim * 4;
   d->off_cut = (d->off_lse + parts * 4 + 15) / 16 * 16;
-  d->bytes = (d->off_cut + 16LL * d->ctas + 255) / 256 * 256;
+  d->off_rows = d->off_cut + 16LL * d->ctas;
+  d->bytes = (d->off_rows + 8LL * d->ctas + 255) / 256 * 256;
   return ATTN_B200_OK;
 }
 
@@ -220,6 +219,7 @@ int paged_setup(const AttnB200PagedAttnArgs* a, const PagedPlan& d, int* status,
   p.part_o = reinterpret_cast<float*>(ws);
   p.part_lse = reinterpret_cast<float*>(ws + d.off_lse);
   p.cut = reinterpret_cast<int4*>(ws + d.off_cut);
+  p.cut_rows = reinterpret_cast<int2*>(ws + d.off_rows);
   p.status = status;
   p.scale = a->scale;
   return ATTN_B200_OK;

@@ -453,8 +453,10 @@ paged_chunk_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant
           else if (p.lse != nullptr) p.lse[(p.cu != nullptr ? static_cast<long long>(head) : static_cast<long long>(u.b) * p.heads + head) * p.seq + at] = lse;
         }
       }
-      if (tid == 0 && !whole && u.t0 == 0)
+      if (tid == 0 && !whole && u.t0 == 0) {
         p.cut[cta] = make_int4(u.b, u.h, u.qt, pg_owner(u.last, share.shares, share.total));
+        p.cut_rows[cta] = make_int2(p.cu != nullptr ? tab.row[u.b] : 0, u.fresh);
+      }
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(bars + L::kOFree + t);

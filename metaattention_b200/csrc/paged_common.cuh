@@ -56,6 +56,7 @@ struct PagedParams {
   float* part_o;                 // [2 * CTAs][D / 4][rows][4]: in paged_chunk.cu a lane has a row (a row's columns in one piece: 4100 cycles a unit)
   float* part_lse;               // [2 * CTAs][rows]
   int4* cut;                     // [CTAs] sequence, KV head, query tile and last CTA of the unit that begins in a CTA and goes on, or w = -1
+  int2* cut_rows;                // [CTAs] first row of that unit's sequence in packed rows (else 0), and its new tokens
   CoordOrder oq, ok, ov;
   int* status;
   float scale;
@@ -567,7 +568,7 @@ struct PagedPlan {
   int group, per_tile, tile_pos, rows, ctas;
   bool few;          // paged_tokens.cu, else paged_chunk.cu
   bool whole;        // units are not cut
-  long long off_lse, off_cut, bytes;
+  long long off_lse, off_cut, off_rows, bytes;
 };
 
 // The launches, by kernel; the tensor maps and parameters of a call are made by paged_setup().

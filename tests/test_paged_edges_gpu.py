@@ -111,3 +111,38 @@ def test_frequencies_outlive_their_embedding_in_a_graph():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want) and len(other) == 400
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# attention over a cache
+# ---------------------------------------------------------------------------------------------------------------
+
+def filled(lens, Hkv, D, page, dtype, codes, seed):
+    """(cache, block_table, cache_seqlens) of random tokens, the pages in random order."""
+    g = torch.Generator().manual_seed(seed)
+    blocks = -(-max(max(lens), 1) // page)
+    cache = PagedKVCache.allocate(len(lens) * blocks, page, Hkv, D, torch.float8_e4m3fn if codes else dtype)
+    table = torch.randperm(len(lens) * blocks, generator=g).view(len(lens), blocks).int().cuda()
+    seqlens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(len(lens), max(lens), Hkv, D, generator=g).to(dtype).cuda() for _ in range(2))
+    full = torch.full_like(seqlens, max(lens))
+    cache.append(k, v, table, full)
+    return cache, table, seqlens
+
+
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("H,lens,rows,backwards,forwards", [(4, [3000, 2000, 2500], 25, [0, 10, 5, 20], [0, 10, 10, 20]), (40, [1500, 700, 1900], 25, [0, 10, 5, 20], [0, 10, 10, 20]),
+                                                            (4, [3000, 2000, 2500], 5, [0, 3, 1, 4], [0, 3, 3, 4]), (4, [300, 200, 250], 5, [0, 3, 1, 4], [0, 3, 3, 4])])
+def test_first_rows_that_go_backwards(codes, H, lens, rows, backwards, forwards):
+    """They count as their predecessors, in units that several blocks share as in whole ones: no row is two sequences'."""
+    cache, table, seqlens = filled(lens, 1, 64, 16, torch.bfloat16, codes, 61)
+    q, n = draw((rows, H, 64), torch.bfloat16, 62).cuda(), forwards[-1]
+    results = []
+    for first in (backwards, forwards):
+        out = torch.full_like(q, 7.0)
+        cu = torch.tensor(first, dtype=torch.int32, device="cuda")
+        o, lse = cache.attention(q, table, seqlens, cu_seqlens=cu, out=out, return_lse=True)
+        assert lib.last_device_status() == 0
+        results.append((o, lse[:, :n]))
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    assert bool((results[0][0][n:] == 7.0).all()) and bool((results[0][0][:n] != 7.0).any(2).all())
