@@ -92,6 +92,6 @@ class PagedKVCache:
         if window is not None and window <= 0:
             raise ValueError(f"window must be positive (got {window})")
         o, lse = native.host().cache_attention(self._native, q, block_table, cache_seqlens, cu_seqlens,
-                                               q.shape[-1] ** -0.5 if scale is None else float(scale), bool(causal),
+                                               self.k.shape[-1] ** -0.5 if scale is None else float(scale), bool(causal),
                                                0 if window is None else int(window), out, return_lse)
         return (o, lse) if return_lse else o

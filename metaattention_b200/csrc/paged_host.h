@@ -398,6 +398,10 @@ std::tuple<Tensor, OptTensor> cache_attention(const Cache& c, const Tensor& q, c
   new_rows(c, q, "q", cu, a.cache.batch, H);
   if (H % Hkv != 0 || H / Hkv > 128) refuse("the ", H, " query heads must be a multiple, of up to 128, of the ", Hkv, " KV heads");
   if (H > 65535) refuse("too many query heads");
+  constexpr int64_t kMost = 0x3fffffff;
+  if (static_cast<int64_t>(a.cache.max_blocks) * a.cache.page_size > kMost)
+    refuse("attention takes sequences of up to 2^30 - 1 tokens (block_table has room for ", a.cache.max_blocks, " blocks of ", a.cache.page_size, ")");
+  if ((cu.has_value() ? 1 : q.size(0)) * q.size(q.dim() - 3) > kMost) refuse("attention takes up to 2^30 - 1 new tokens, got q ", shape_of(q));
   if (a.cache.batch > 1024) refuse("at most 1024 sequences (got ", a.cache.batch, ")");
   if (!(scale > 0.0) || !std::isfinite(static_cast<float>(scale)) || static_cast<float>(scale) == 0.0f) refuse("scale must be positive and finite (got ", scale, ")");
   if (window < 0) refuse("window must be positive (got ", window, ")");
@@ -410,32 +414,46 @@ std::tuple<Tensor, OptTensor> cache_attention(const Cache& c, const Tensor& q, c
     for (int64_t d = 0; d < out->dim(); ++d)
       if (out->size(d) > 1 && out->stride(d) == 0) refuse("every value of out must have memory of its own (an expanded tensor has not)");
   }
+  const int64_t seq = q.size(q.dim() - 3);
+  a.cu_seqlens = cu.has_value() ? cu->data_ptr<int32_t>() : nullptr;
+  a.heads = H;
+  a.seq = seq;
+  a.dtype = dtype_code(q);
+  a.scale = static_cast<float>(scale);
+  a.causal = causal;
+  a.window = static_cast<int32_t>(std::min<int64_t>(window, kMost));
+  c10::cuda::CUDAGuard guard(q.device());
+  int64_t need = 0;
+  if (q.numel() > 0) {
+    need = paged_api.bytes(&a);   // all but the length of the list of work has been looked at above
+    if (need < 0) refuse("the call is too long: ", a.cache.batch, " sequences of up to ", a.cache.max_blocks, " blocks, q ", shape_of(q));
+  }
   py::gil_scoped_release others_run;
   at::AutoDispatchBelowADInplaceOrView below;
-  c10::cuda::CUDAGuard guard(q.device());
   Tensor o = out.has_value() ? *out : fresh(q.sizes(), q.scalar_type(), q);
-  const int64_t seq = q.size(q.dim() - 3);
   OptTensor lse;
   if (want_lse) lse = cu.has_value() ? fresh({H, seq}, at::kFloat, q) : fresh({q.size(0), H, seq}, at::kFloat, q);
   if (q.numel() == 0) return {o, lse};
   a.q = q.data_ptr();
   a.o = o.data_ptr();
   a.lse = want_lse ? lse->data_ptr<float>() : nullptr;
-  a.cu_seqlens = cu.has_value() ? cu->data_ptr<int32_t>() : nullptr;
   row_strides(a.q_stride, q);
   row_strides(a.o_stride, o);
-  a.heads = H;
-  a.seq = seq;
-  a.dtype = dtype_code(q);
-  a.scale = static_cast<float>(scale);
-  a.causal = causal;
-  a.window = static_cast<int32_t>(std::min<int64_t>(window, 0x3fffffff));
-  const int64_t need = paged_api.bytes(&a);
-  if (need < 0) check(ATTN_B200_E_UNSUPPORTED, "attn_b200_paged_workspace_bytes");
   Tensor ws = fresh({std::max<int64_t>(need, 16)}, at::kByte, q);
   a.workspace = ws.data_ptr();
   a.workspace_bytes = ws.numel();
-  check(paged_api.attention(&a, stream_of(q)), "attn_b200_paged_attention");
+  int rc = paged_api.attention(&a, stream_of(q));
+  Tensor own;
+  if (rc == ATTN_B200_E_UNSUPPORTED) {   // q in memory that several values share, for a kernel whose loads have no stride of zero: nothing was launched
+    for (int64_t d = 0; d < q.dim() && !own.defined(); ++d)
+      if (q.size(d) > 1 && q.stride(d) == 0) own = q.contiguous();
+    if (own.defined()) {
+      a.q = own.data_ptr();
+      row_strides(a.q_stride, own);
+      rc = paged_api.attention(&a, stream_of(q));
+    }
+  }
+  check(rc, "attn_b200_paged_attention");
   if (out.has_value() && !o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
   return {o, lse};
 }

@@ -146,3 +146,35 @@ def test_first_rows_that_go_backwards(codes, H, lens, rows, backwards, forwards)
         results.append((o, lse[:, :n]))
     assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
     assert bool((results[0][0][n:] == 7.0).all()) and bool((results[0][0][:n] != 7.0).any(2).all())
+
+
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("n", [1, 3, 70])
+@pytest.mark.parametrize("axis", [0, 1, 2])
+def test_queries_in_memory_that_several_share(codes, n, axis):
+    """q expanded over sequences, positions or heads: as its copy, whichever kernel it takes; packed too."""
+    cache, table, seqlens = filled([300, 90, 1000], 2, 64, 16, torch.float16, codes, 63)
+    shape = [3, n, 4, 64]
+    q = draw([1 if i == axis else x for i, x in enumerate(shape)], torch.float16, 64).cuda().expand(shape)
+    got, want = (cache.attention(t, table, seqlens, return_lse=True) for t in (q, q.clone(memory_format=torch.contiguous_format)))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    if axis > 0:
+        cu = torch.tensor([0, 0, n, n], dtype=torch.int32, device="cuda")
+        packed = q[1]
+        got, want = (cache.attention(t, table, seqlens, cu_seqlens=cu, return_lse=True) for t in (packed, packed.clone(memory_format=torch.contiguous_format)))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert lib.last_device_status() == 0
+
+
+def test_sizes_beyond_the_kernels_are_refused_by_name():
+    """Before anything is launched or allocated: the operands are one row in the place of many."""
+    cache = PagedKVCache.allocate(1, 1 << 20, 1, 64, torch.float8_e4m3fn)
+    lens = torch.ones(1, dtype=torch.int32, device="cuda")
+    q = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    for blocks, seq, word in ((1024, 1, "2\\^30 - 1 tokens"), (1, 1 << 30, "2\\^30 - 1 new tokens"), (512, 1 << 20, "too long")):
+        table = torch.zeros(1, blocks, dtype=torch.int32, device="cuda")
+        with pytest.raises(ValueError, match=word):
+            cache.attention(q.expand(1, seq, 1, 64), table, lens)
+    for bad in (q[..., :0], q[..., :32], q[0, 0, 0, 0]):
+        with pytest.raises(ValueError):
+            cache.attention(bad, table, lens)
