@@ -495,8 +495,9 @@ typedef struct AttnB200PagedReadArgs {
 int attn_b200_paged_read(const AttnB200PagedReadArgs* args, void* cuda_stream);
 
 /* Attention of the new tokens of each sequence over what its pages hold, softmax(scale * Q.K^T).V with grouped heads: row at
- * position p (the new tokens are the last ones) sees the keys at p and in front of it (causal = 1; 0: all), with window > 0
- * only those from p - window + 1 on.  A row that sees none gives 0 and -inf.  q, o: [batch, seq, heads, head_dim], or with
+ * position p (the new tokens are the last ones) sees the keys at p and in front of it, with window > 0 only those from
+ * p - window + 1 on (causal = 1), or all keys of its sequence, also where p is negative (causal = 0).  A row that sees none gives 0
+ * and -inf.  q, o: [batch, seq, heads, head_dim], or with
  * cu_seqlens packed rows [seq, heads, head_dim] as in AttnB200PagedAppendArgs; packed rows behind cu_seqlens[batch] are left
  * as they are.  An 8-bit cache is read as the 16-bit values of q's type that its codes stand for.  At most 1024 sequences,
  * 128 query heads to a KV head. */

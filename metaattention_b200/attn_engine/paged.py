@@ -83,12 +83,12 @@ class PagedKVCache:
                   return_lse: bool = False):
         """Softmax attention of the new tokens' q [.., heads, head_dim] over their sequences' keys, ``heads`` a multiple of
         heads_kv (query head h reads KV head h // (heads / heads_kv)): o like q, and with ``return_lse`` (o, lse), lse the
-        log-sum-exp of each row in float32 [batch, heads, seq], packed [heads, rows].  The row at position p sees the keys up to
-        its own (``causal``; else all), with ``window`` only the last ``window`` of those; a row that sees none, as one at a
-        negative position, gives 0 and -inf.  ``scale`` defaults to head_dim ** -0.5.  Written to ``out`` if given; packed rows
-        behind the last sequence are left as they are there (and are not initialised otherwise).  An 8-bit cache is read as
-        the values of q's dtype that its codes stand for.  Keys and values inside a sequence must be finite; what lies behind
-        its end is not looked at.  No backward pass, and no forward-mode one."""
+        log-sum-exp of each row in float32 [batch, heads, seq], packed [heads, rows].  With ``causal`` the row at position p sees the
+        keys up to its own, with ``window`` only the last ``window`` of those, at a negative position none; without, every row sees
+        all keys of its sequence, wherever it is.  A row that sees none gives 0 and -inf.  ``scale`` defaults to head_dim ** -0.5.
+        Written to ``out`` if given; packed rows behind the last sequence are left as they are there (and are not initialised
+        otherwise).  An 8-bit cache is read as the values of q's dtype that its codes stand for.  Keys and values inside a sequence
+        must be finite; what lies behind its end is not looked at.  No backward pass, and no forward-mode one."""
         if window is not None and window <= 0:
             raise ValueError(f"window must be positive (got {window})")
         o, lse = native.host().cache_attention(self._native, q, block_table, cache_seqlens, cu_seqlens,

@@ -178,3 +178,17 @@ def test_sizes_beyond_the_kernels_are_refused_by_name():
     for bad in (q[..., :0], q[..., :32], q[0, 0, 0, 0]):
         with pytest.raises(ValueError):
             cache.attention(bad, table, lens)
+
+
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("n", [3, 70])
+def test_rows_at_negative_positions(codes, n):
+    """More new tokens than tokens: causal rows in front of the sequence see nothing, others see every key."""
+    cache, table, seqlens = filled([2, 0, 300], 1, 64, 16, torch.bfloat16, codes, 65)
+    q = draw((3, 1, 2, 64), torch.bfloat16, 66).expand(3, n, 2, 64).contiguous().cuda()
+    o, lse = cache.attention(q, table, seqlens, return_lse=True)
+    assert bool((o[0, :n - 2] == 0).all()) and bool((lse[0, :, :n - 2] == -torch.inf).all()) and bool(lse[0, :, n - 2:].isfinite().all())
+    o, lse = cache.attention(q, table, seqlens, causal=False, return_lse=True)
+    for b in (0, 2):   # the same query everywhere: the same row everywhere
+        assert torch.equal(o[b], o[b, -1:].expand_as(o[b])) and bool(lse[b].isfinite().all())
+    assert bool((o[1] == 0).all()) and bool((lse[1] == -torch.inf).all())
