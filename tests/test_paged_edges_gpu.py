@@ -9,6 +9,7 @@ import torch
 
 from attn_engine import PagedKVCache, RotaryEmbedding
 from core.native import lib
+from oracle import paged_math as pm
 
 pytestmark = pytest.mark.gpu
 
@@ -192,3 +193,62 @@ def test_rows_at_negative_positions(codes, n):
     for b in (0, 2):   # the same query everywhere: the same row everywhere
         assert torch.equal(o[b], o[b, -1:].expand_as(o[b])) and bool(lse[b].isfinite().all())
     assert bool((o[1] == 0).all()) and bool((lse[1] == -torch.inf).all())
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# what a cache holds
+# ---------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("codes", [False, True])
+def test_a_cache_holds_the_turned_keys_and_the_values(codes):
+    """Step by step as a server appends, against the rows that were given, turned by their positions in 64 bits.  16 bits: keys as in
+    test_rotary_gpu.py, values equal.  8 bits: half a step of the code (2^-4 of the value, or 2^-16 of the row's largest where codes are
+    subnormal: half of 2^-9 steps of 2^e, 2^e < largest / 224), plus for keys what the angle may be off, twice where the code flips."""
+    Hkv, D, page, dtype = 2, 64, 16, torch.bfloat16
+    cache = PagedKVCache.allocate(20, page, Hkv, D, torch.float8_e4m3fn if codes else dtype)
+    rope = RotaryEmbedding(D, base=5000.0)
+    table = torch.randperm(20, generator=torch.Generator().manual_seed(71))[:14].view(2, 7).int().cuda()
+    rows = {(w, b): [] for w in "kv" for b in (0, 1)}
+    total = [0, 0]
+    for step, news in enumerate(([60, 17], [23, 41], [1, 1], [0, 1], [1, 0])):
+        total = [a + b for a, b in zip(total, news)]
+        lens, cu = torch.tensor(total, dtype=torch.int32).cuda(), torch.tensor([0, news[0], sum(news)], dtype=torch.int32).cuda()
+        k, v = (draw((sum(news), Hkv, D), dtype, 72 + 2 * step + i) for i in (0, 1))
+        cache.append(k.cuda(), v.cuda(), table, lens, cu_seqlens=cu, rotary=rope)
+        for w, x in (("k", k), ("v", v)):
+            for b, part in enumerate(x.split(news)):
+                rows[w, b].append(part)
+        kk, vv = (t.cpu().double() for t in cache.read(table, lens, max(total)))
+        for b in (0, 1):
+            given = torch.cat(rows["k", b])
+            want = pm.rotary(given, torch.arange(total[b]), rope.frequencies)
+            pair = (given[..., :D // 2].double().abs() + given[..., D // 2:].double().abs()).repeat(1, 1, 2) * 2.0 ** -20
+            values = torch.cat(rows["v", b]).double()
+            if codes:
+                def half(x):
+                    return torch.maximum(x.abs() * 2.0 ** -4, x.abs().amax(-1, keepdim=True) * 2.0 ** -16)
+                assert bool(((kk[b, :total[b]] - want).abs() <= half(want) + 2 * pair).all())
+                assert bool(((vv[b, :total[b]] - values).abs() <= half(values)).all())
+            else:
+                assert bool(((kk[b, :total[b]] - want).abs() <= want.abs() * 2.0 ** -8 + pair).all())
+                assert torch.equal(vv[b, :total[b]], values)
+            if total[b] > 1:   # a tolerance that tells: the rows as they were given are outside of it
+                assert bool(((kk[b, :total[b]] - given.double()).abs() > 0.5).any())
+    assert lib.last_device_status() == 0
+
+
+def test_codes_that_are_written_again_stay():
+    """Reading codes back and writing them gives the same codes and scales; a row whose largest code is 224 may take the next smaller
+    scale (448 of it is the same value), with codes of twice the value."""
+    cache, table, lens = filled([77, 77], 2, 128, 16, torch.bfloat16, True, 74)
+    before = [t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    a, b = cache.read(table, lens, 77)
+    cache.append(a, b, table, lens)
+    for i, values in ((0, a), (1, b)):
+        pool, scale = (cache.k, cache.k_scale) if i == 0 else (cache.v, cache.v_scale)
+        borderline = before[i].float().abs().amax(-1) == 224
+        assert int(borderline.sum()) < borderline.numel() // 4
+        assert torch.equal(pool.view(torch.uint8)[~borderline], before[i].view(torch.uint8)[~borderline])
+        assert torch.equal(scale.view(torch.uint8)[~borderline], before[2 + i].view(torch.uint8)[~borderline])
+        assert torch.equal(cache.read(table, lens, 77)[i], values)
+    assert lib.last_device_status() == 0
