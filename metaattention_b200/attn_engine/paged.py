@@ -23,7 +23,8 @@ class PagedKVCache:
     with ``k_scale``, ``v_scale`` [num_pages, page_size, heads_kv] (float8_e8m0fnu, or uint8 exponents): a code stands for
     code * 2^(exponent - 127), a row of exponent 255 for NaN; the codes 0x7f and 0xff belong to such rows alone.
     Any strides of whole 16 bytes with a contiguous last dimension; page_size a power of two of at least 8, head_dim 64 or 128.
-    The pools are the caller's tensors and are written in place.
+    The pools are the caller's tensors and are written in place; they stay where they are (a call after one was resized or given
+    other memory is refused).
 
     Common arguments: ``block_table`` int32 [batch, max_blocks] names the page of each page_size tokens of a sequence (entries
     behind its end may hold anything); ``cache_seqlens`` int32 [batch], tokens of each sequence with the new ones among them, at
@@ -33,15 +34,20 @@ class PagedKVCache:
     of them on the cache's device; calls run on the current stream of that device."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self._native = native.host().make_cache(k, v, k_scale, v_scale)
+        self._pools = (k, v, k_scale, v_scale)
+        self._native = native.host().make_cache(*self._pools)
 
     def __getstate__(self):
         return {**self.__dict__, "_native": None}
 
     def __setstate__(self, state):
         self.__dict__.update(state)
-        self._native = native.host().make_cache(self.k, self.v, self.k_scale, self.v_scale)
+        self._native = native.host().make_cache(*self._pools)
+
+    k = property(lambda self: self._pools[0])
+    v = property(lambda self: self._pools[1])
+    k_scale = property(lambda self: self._pools[2])
+    v_scale = property(lambda self: self._pools[3])
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, heads_kv: int, head_dim: int, dtype=torch.bfloat16, device="cuda"):

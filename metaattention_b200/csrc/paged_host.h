@@ -229,6 +229,7 @@ std::vector<Tensor> rotary_call(const std::shared_ptr<const Turns>& turns, const
 
 struct Cache {
   Tensor k, v, k_scale, v_scale;
+  std::vector<int64_t> shape;   // of the pools
   AttnB200PagedCache view;
 };
 
@@ -268,6 +269,7 @@ std::shared_ptr<Cache> make_cache(const Tensor& k, const Tensor& v, const OptTen
   }
   c->k = k;
   c->v = v;
+  c->shape = k.sizes().vec();
   AttnB200PagedCache& a = c->view;
   a.k = k.data_ptr();
   a.v = v.data_ptr();
@@ -289,6 +291,15 @@ std::shared_ptr<Cache> make_cache(const Tensor& k, const Tensor& v, const OptTen
 
 // The sequences of a call; `held` keeps a copy alive until its launch.
 AttnB200PagedCache sequences(const Cache& c, const Tensor& table, const Tensor& lens, Tensor& held) {
+  // a pool whose tensor was resized or given other memory since the cache was made: its pages are no longer where the view says
+  bool same = c.k.dim() == 4 && c.v.dim() == 4 && c.k.data_ptr() == c.view.k && c.v.data_ptr() == c.view.v && c.k.sizes() == c.shape && c.v.sizes() == c.shape;
+  for (int i = 0; same && i < 3; ++i) same = c.k.stride(i) == c.view.k_stride[i] && c.v.stride(i) == c.view.v_stride[i];
+  if (same && c.view.k_scale != nullptr) {
+    const at::IntArrayRef rows(c.shape.data(), 3);
+    same = c.k_scale.data_ptr() == c.view.k_scale && c.v_scale.data_ptr() == c.view.v_scale && c.k_scale.sizes() == rows && c.v_scale.sizes() == rows;
+    for (int i = 0; same && i < 3; ++i) same = c.k_scale.stride(i) == c.view.k_scale_stride[i] && c.v_scale.stride(i) == c.view.v_scale_stride[i];
+  }
+  if (!same) refuse("the pools have other memory or another shape than when the PagedKVCache was made: make a new one");
   if (!c.k.is_cuda()) refuse("the cache is not on a CUDA device");
   if (table.scalar_type() != at::kInt || table.dim() != 2) refuse("block_table must be an int32 tensor [batch, max_blocks], got ", table.scalar_type(), " ", shape_of(table));
   if (lens.scalar_type() != at::kInt || lens.dim() != 1 || lens.size(0) != table.size(0))

@@ -38,3 +38,34 @@ def test_tangents_of_forward_mode_are_refused():
                 call()
         with forward_ad._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="CUDA"):   # the next refusal
             cache.attention(dual16, table, lens)
+
+
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("which", ["k", "v", "k_scale", "v_scale"])
+@pytest.mark.parametrize("how", ["data", "resized", "emptied", "shape"])
+def test_pools_that_moved_are_refused(codes, which, how):
+    """The native side knows where the pages were; it must not read there when they are not any more."""
+    if not codes and "scale" in which:
+        return
+    kind = torch.float8_e4m3fn if codes else torch.bfloat16
+    made = [torch.zeros(4, 16, 2, 64, dtype=kind) for _ in range(2)] + ([torch.zeros(4, 16, 2, dtype=torch.uint8) for _ in range(2)] if codes else [])
+    cache, table, lens = PagedKVCache(*made), torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    q = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16)
+    calls = [lambda: cache.read(table, lens, 4), lambda: cache.attention(q, table, lens), lambda: cache.append(q, q, table, lens)]
+    for call in calls:
+        with pytest.raises(ValueError, match="CUDA"):   # the first refusal, as long as they are there
+            call()
+    pool = getattr(cache, which)
+    if how == "data":
+        pool.data = pool.clone()
+    elif how == "resized":
+        pool.resize_(8, *pool.shape[1:])
+    elif how == "emptied":
+        pool.untyped_storage().resize_(0)
+    else:
+        pool.data = pool.data.view(8, 8, *pool.shape[2:])
+    for call in calls:
+        with pytest.raises(ValueError, match="make a new one"):
+            call()
+    with pytest.raises(AttributeError):
+        cache.k = made[0]
