@@ -70,7 +70,8 @@ class PagedKVCache:
         bits) to the last positions of their sequences.  8 bits: a scale for each token and head, the least power of two that
         brings its largest magnitude to 448 at most; a row with a value that is not finite becomes NaN.  ``rotary`` (a
         RotaryEmbedding with a rotary_dim that is a multiple of 16) turns k by its positions on the way, rounded once.  Tokens at
-        negative positions, and those whose table entry names no page, are not written; no two may have the same place."""
+        negative positions, and those whose table entry names no page, are not written; no two may have the same place, nor may the
+        pools k and v be one."""
         turns = None
         if rotary is not None and self.k.is_cuda:
             turns = rotary.native_on(self.k.device)

@@ -346,6 +346,7 @@ void cache_append(const Cache& c, const Tensor& k, const Tensor& v, const Tensor
   std::memset(&a, 0, sizeof(a));
   Tensor held;
   no_tangent("a cache", {&k, &v, &c.k, &c.v});
+  if (c.view.k == c.view.v || (c.view.k_scale != nullptr && c.view.k_scale == c.view.v_scale)) refuse("the k and v of a cache that is written must not be the same memory");
   a.cache = sequences(c, table, lens, held);
   new_rows(c, k, "k", cu, a.cache.batch, a.cache.heads_kv);
   new_rows(c, v, "v", cu, a.cache.batch, a.cache.heads_kv);

@@ -69,3 +69,16 @@ def test_pools_that_moved_are_refused(codes, which, how):
             call()
     with pytest.raises(AttributeError):
         cache.k = made[0]
+
+
+@pytest.mark.parametrize("codes", [False, True])
+def test_one_pool_for_keys_and_values_is_not_written(codes):
+    """Attention may read one pool as both; what an append left in it would be either."""
+    kind, scale = (torch.float8_e4m3fn, torch.zeros(4, 16, 2, dtype=torch.uint8)) if codes else (torch.bfloat16, None)
+    pool, other = (torch.zeros(4, 16, 2, 64, dtype=kind) for _ in range(2))
+    table, lens, k = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32), torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16)
+    for cache in [PagedKVCache(pool, pool, scale, scale)] + ([PagedKVCache(pool, other, scale, scale)] if codes else []):
+        with pytest.raises(ValueError, match="same memory"):
+            cache.append(k, k, table, lens)
+        with pytest.raises(ValueError, match="CUDA"):
+            cache.attention(k, table, lens)
