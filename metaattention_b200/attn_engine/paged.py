@@ -21,7 +21,9 @@ from core.native import lib as native
 class PagedKVCache:
     """Pools of pages ``k``, ``v`` [num_pages, page_size, heads_kv, head_dim] in float16, bfloat16 or float8_e4m3fn, the last
     with ``k_scale``, ``v_scale`` [num_pages, page_size, heads_kv] (float8_e8m0fnu, or uint8 exponents): a code stands for
-    code * 2^(exponent - 127), a row of exponent 255 for NaN; the codes 0x7f and 0xff belong to such rows alone.
+    code * 2^(exponent - 127), a row of exponent 255 for NaN.  The codes 0x7f and 0xff belong to such rows alone, as ``append`` writes
+    them: in other rows ``read`` gives NaN for them, and ``attention``, which does not look for them, may take them for 480 times the
+    scale.
     Any strides of whole 16 bytes with a contiguous last dimension; page_size a power of two of at least 8, head_dim 64 or 128.
     The pools are the caller's tensors and are written in place; they stay where they are (a call after one was resized or given
     other memory is refused).
