@@ -94,11 +94,11 @@ class RotaryEmbedding:
         made = self._turns.get(device)
         if made is None:
             index = device.index if device.index is not None else torch.cuda.current_device()
-            if torch.cuda.is_current_stream_capturing():
-                raise native.NativeError("the first call of a RotaryEmbedding on a device lays its frequencies out there: make it before the capture")
-            with torch.inference_mode(False):
+            with torch.cuda.device(index), torch.inference_mode(False):   # the stream that is asked and waited for is that device's
+                if torch.cuda.is_current_stream_capturing():
+                    raise native.NativeError("the first call of a RotaryEmbedding on a device lays its frequencies out there: make it before the capture")
                 table = torch.tensor(self._table, dtype=torch.int64).to(torch.device("cuda", index))
-            torch.cuda.current_stream(index).synchronize()   # other streams use it too
+                torch.cuda.current_stream().synchronize()   # other streams use it too
             made = self._turns[device] = native.host().make_turns(table, self.rotary_dim, self.interleaved, self.magnitude)
         return made
 

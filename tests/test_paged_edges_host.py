@@ -5,7 +5,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from attn_engine import PagedKVCache
+from attn_engine import PagedKVCache, RotaryEmbedding
 from core.native import lib
 
 
@@ -82,3 +82,23 @@ def test_one_pool_for_keys_and_values_is_not_written(codes):
             cache.append(k, k, table, lens)
         with pytest.raises(ValueError, match="CUDA"):
             cache.attention(k, table, lens)
+
+
+def test_frequencies_ask_their_own_device_for_a_capture(monkeypatch):
+    """A call on a device that is not the current one: the capture that counts is under way there, or not at all."""
+    current, capturing = [0], {1}
+
+    class On:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[0] in capturing)
+    with pytest.raises(lib.NativeError, match="before the capture"):
+        RotaryEmbedding(8).native_on(torch.device("cuda", 1))
+    assert current == [0]
