@@ -32,6 +32,11 @@ bool wide_strides(const Tensor& t, int64_t unit) {   // whole 16-byte pieces
   return t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
+// A tensor without memory (its storage freed, or zeros that stand for themselves) has an address that must not be read.
+void has_memory(const char* what, const Tensor& t) {
+  if (!t.unsafeGetTensorImpl()->storage_initialized()) refuse(what, " ", shape_of(t), " has no memory");
+}
+
 // A tangent of forward mode beside the values: these launches would leave it behind without a word.
 void no_tangent(const char* what, std::initializer_list<const Tensor*> given) {
   for (const Tensor* t : given)
@@ -167,7 +172,8 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     for (size_t i = 0; i < grads.size(); ++i)
       if (grads[i].defined() && ctx->needs_input_grad((saved.defined() ? 1 : 0) + i)) {   // counted over the tensors of the call
         which.push_back(static_cast<int>(i));
-        g.push_back(grads[i].stride(-1) == 1 || grads[i].numel() == 0 ? grads[i] : grads[i].contiguous());
+        const bool zeros = grads[i]._is_zerotensor();   // without memory of their own
+        g.push_back(zeros ? at::zeros(grads[i].sizes(), grads[i].options()) : grads[i].stride(-1) == 1 || grads[i].numel() == 0 ? grads[i] : grads[i].contiguous());
       }
     if (g.empty()) return out;
     c10::cuda::CUDAGuard guard(g[0].device());
@@ -194,12 +200,14 @@ std::vector<Tensor> rotary_call(const std::shared_ptr<const Turns>& turns, const
   }
   for (const Tensor& t : x) {
     no_tangent("a rotation by positions", {&t});
+    has_memory("a tensor of heads", t);
     if (t.numel() > 0 && t.stride(-1) != 1) refuse("the last dimension must be contiguous");
   }
   if (positions.has_value()) {
     const Tensor& p = *positions;
     if (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong) refuse("positions must be int32 or int64 (got ", p.scalar_type(), ")");
     if (p.device() != q.device()) refuse("positions must be on the device of q");
+    has_memory("positions", p);
     const bool shared = p.dim() == 1 && p.size(0) == q.size(lead - 1);
     const bool each = p.dim() == 2 && lead == 2 && (p.size(0) == q.size(0) || p.size(0) == 1) && p.size(1) == q.size(1);
     if (!shared && !each) refuse("positions must be [seq] or [batch, seq] for q ", shape_of(q), ", got ", shape_of(p));
@@ -247,6 +255,7 @@ std::shared_ptr<Cache> make_cache(const Tensor& k, const Tensor& v, const OptTen
   if (page < 8 || (page & (page - 1)) != 0) refuse("page_size must be a power of two of at least 8 (got ", page, ")");
   if (k.size(0) > 0x7fffffff || page > 0x40000000 || k.size(2) > 65535) refuse("the pools are too large");
   for (const Tensor* t : {&k, &v}) {
+    has_memory("a pool", *t);
     if (!wide_strides(*t, codes ? 16 : 8)) refuse("the pools need a contiguous last dimension, and strides and addresses of whole 16 bytes");
     for (int i = 0; i < 3; ++i)
       if (t->size(i) > 1 && t->stride(i) <= 0) refuse("the pools need positive strides");
@@ -259,6 +268,7 @@ std::shared_ptr<Cache> make_cache(const Tensor& k, const Tensor& v, const OptTen
       if (s.dim() != 3 || s.size(0) != k.size(0) || s.size(1) != page || s.size(2) != k.size(2))
         refuse("scales must be [num_pages, page_size, heads_kv] for pools ", shape_of(k), ", got ", shape_of(s));
       if (s.device() != k.device()) refuse("pools and scales must be on one device");
+      has_memory("a pool of scales", s);
       for (int i = 0; i < 3; ++i)
         if (s.size(i) > 1 && s.stride(i) <= 0) refuse("scales need positive strides");
     }
@@ -328,6 +338,7 @@ void new_rows(const Cache& c, const Tensor& t, const char* what, const OptTensor
   if (dtype_code(t) < 0 || (c.view.dtype != ATTN_B200_DTYPE_E4M3 && t.scalar_type() != c.k.scalar_type()))
     refuse(what, " must be float16 or bfloat16, and the dtype of a 16-bit cache (got ", t.scalar_type(), ")");
   if (t.size(packed ? 0 : 1) > 0x7fffffff || (!packed && t.size(0) * t.size(1) > 0x7fffffff)) refuse(what, " has too many rows");
+  has_memory(what, t);
   if (t.numel() > 0 && !wide_strides(t, 8)) refuse(what, " needs a contiguous last dimension, and strides and address of whole 16 bytes");
   if (packed && (cu->scalar_type() != at::kInt || cu->dim() != 1 || cu->size(0) != batch + 1 || (batch > 0 && cu->stride(0) != 1) || cu->device() != c.k.device()))
     refuse("cu_seqlens must be a contiguous int32 tensor [batch + 1] on the device of the cache");

@@ -73,6 +73,29 @@ def test_only_what_asks_for_a_gradient_gets_one(given, both):
             assert torch.equal(cache.read(table, lens, 5)[0], b)
 
 
+def test_tensors_without_memory_are_refused():
+    """Before anything is launched; a gradient of zeros that has none is zeros."""
+    cache, table, lens = filled([30, 20], 2, 64, 16, torch.bfloat16, False, 9)
+
+    def freed(*shape, dtype=torch.bfloat16):
+        t = torch.zeros(2, *shape, dtype=dtype, device="cuda")[1]
+        t.untyped_storage().resize_(0)
+        return t
+    q, kv = torch.zeros(2, 1, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 1, 2, 64, dtype=torch.bfloat16, device="cuda")
+    for call in (lambda: RotaryEmbedding(64)(freed(2, 1, 2, 64)), lambda: cache.attention(freed(2, 1, 2, 64), table, lens),
+                 lambda: cache.attention(q, table, lens, out=freed(2, 1, 2, 64)), lambda: cache.append(freed(2, 1, 2, 64), kv, table, lens),
+                 lambda: cache.append(kv, freed(2, 1, 2, 64), table, lens)):
+        with pytest.raises(ValueError, match="no memory"):
+            call()
+    for args in ((freed(2, 2, dtype=torch.int32), lens, None), (table, freed(2, dtype=torch.int32), None), (table, lens, freed(3, dtype=torch.int32))):
+        with pytest.raises((ValueError, RuntimeError)):
+            cache.attention(q[:, 0] if args[2] is not None else q, *args)
+    leaf = torch.ones(2, 3, 2, 64, device="cuda", requires_grad=True)
+    y = RotaryEmbedding(64)(leaf)
+    (d,) = torch.autograd.grad(y, leaf, torch._efficientzerotensor(2, 3, 2, 64, device="cuda"))
+    assert bool((d == 0).all())
+
+
 def overwrite_what_is_free():
     """Blocks of the size of a small table, from the current stream's memory, with other contents."""
     return [torch.full((n,), -(2 ** 61) + 12345, dtype=torch.int64, device="cuda") for n in (32, 64) for _ in range(200)]

@@ -102,3 +102,21 @@ def test_frequencies_ask_their_own_device_for_a_capture(monkeypatch):
     with pytest.raises(lib.NativeError, match="before the capture"):
         RotaryEmbedding(8).native_on(torch.device("cuda", 1))
     assert current == [0]
+
+
+def freed(*shape, dtype=torch.bfloat16):
+    """A tensor whose storage was given back, as sharded training does between layers; not at the storage's begin."""
+    t = torch.zeros(2, *shape, dtype=dtype)[1]
+    t.untyped_storage().resize_(0)
+    return t
+
+
+def test_tensors_without_memory_are_refused():
+    x, pos = torch.zeros(2, 1, 2, 64), torch.arange(1)
+    calls = [lambda: rotary(freed(2, 1, 2, 64), None, None, False), lambda: rotary(x, freed(2, 1, 2, 64, dtype=torch.float32), None, False),
+             lambda: rotary(x, None, freed(1, dtype=torch.int64), False), lambda: rotary(torch._efficientzerotensor(2, 1, 2, 64), None, pos, False),
+             lambda: PagedKVCache(freed(4, 16, 2, 64), pools()[1]), lambda: PagedKVCache(pools()[0], freed(4, 16, 2, 64)),
+             lambda: PagedKVCache(*pools(dtype=torch.float8_e4m3fn), torch.zeros(4, 16, 2, dtype=torch.uint8), freed(4, 16, 2, dtype=torch.uint8))]
+    for call in calls:
+        with pytest.raises(ValueError, match="no memory"):
+            call()
