@@ -92,14 +92,13 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
   }
   const long long in_b = p.cu == nullptr ? b : 0;
   uint4 lo[2], hi[2];
-  // read once, and first to leave the L2 cache: the pages stay, for the attention that reads them (4 x 2048 prompts 14.8 -> 13.7 us)
   auto load = [&](int h, uint4 (&lo)[2], uint4 (&hi)[2]) {
     if (live && h < p.c.heads) {
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const uint16_t* src = p.in[w] + in_b * p.is[w][0] + t * p.is[w][1] + h * p.is[w][2];
-        lo[w] = __ldcs(reinterpret_cast<const uint4*>(src + (w == 0 ? c0 : unit * 16)));
-        hi[w] = __ldcs(reinterpret_cast<const uint4*>(src + (w == 0 ? c1 : unit * 16 + 8)));
+        lo[w] = *reinterpret_cast<const uint4*>(src + (w == 0 ? c0 : unit * 16));
+        hi[w] = *reinterpret_cast<const uint4*>(src + (w == 0 ? c1 : unit * 16 + 8));
       }
     }
   };
