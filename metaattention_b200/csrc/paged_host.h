@@ -39,6 +39,7 @@ void has_memory(const char* what, const Tensor& t) {
 
 // A tangent of forward mode beside the values: these launches would leave it behind without a word.
 void no_tangent(const char* what, std::initializer_list<const Tensor*> given) {
+  if (torch::autograd::ForwardADLevel::try_get_by_idx(0) == nullptr) return;   // no dual level is open
   for (const Tensor* t : given)
     if (t->_fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
       refuse(what, " has no forward-mode derivative (torch.autograd.forward_ad): a tensor of the call carries a tangent");
