@@ -9,9 +9,12 @@
 //   four warps       loads of K and Q, of V; issue S = Q K^T, O += P V: with one warp for both its waits and bookkeeping stood in
 //                    front of an idle pipe, 2130 cycles for a tile of 128 x 128 where the pipe needs 1024
 //   eight more       8-bit caches: exponents of the rows; K and V in 16 bits (paged_common.cuh)
-// Measured: twice 1024 new tokens on 16384, 32 heads on 8 KV heads of 128: 506-552 us at the capped clock (1.35 GHz), 965-1050
-// TFLOP/s; 64 columns 390; 8 bits 700.  A step (a KV tile, both query tiles) is 2100 cycles where nothing is masked, 2048 of them
-// exponentials, up to 3000 in short units; a unit's beginning and end 4000 to 6000.
+// P is rounded to q's type, the operand's; its sum is taken of the unrounded values, in 32 bits.  (Error of o against 64 bits, relative
+// in the norm: 0.0023 in bf16 where the rounding of o alone gives 0.0017, as in the dense kernels; a P in two parts would double P V.)
+// Measured: twice 1024 new tokens on 16384, 32 heads on 8 KV heads of 128: 557-568 us behind one another, at the capped clock (1.36 GHz),
+// 940-955 TFLOP/s; 64 columns 384-390; 8 bits 694-700, 64 columns 550.  A step (a KV tile, both query tiles) is 3100 cycles of that
+// call (670 k for 215 steps): each of the tensor pipe and the special-function unit needs 2048 of them and neither is full (63 and 67 %);
+// a step of one query tile is 2100, the chain of scores, exponentials, P and product; a unit's beginning and end 4000 to 6000.
 #include <cstring>
 
 #include "paged_common.cuh"

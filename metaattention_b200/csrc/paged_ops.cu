@@ -6,8 +6,9 @@
 //            A power of two loses nothing against a scale of amax / 448 (the codes are floating point, their relative step is
 //            the same anywhere in the range), divides exactly and makes code * 2^e exact in 16 bits again.
 //   read:    the rows of each sequence one after the other, code * 2^e rounded once to 16 bits, zeros behind the end.
-// Measured: 4 x 2048 tokens of 8 heads of 128, turned, into 16-bit pages 13.7 us = 4.9 TB/s; 64 single tokens in 8 bits 3.7 us, of which
-// 3.3 are the host's; 8 sequences of up to 8192 tokens out of 8 bits 68 us = 5.4 TB/s (a copy's rate: 6.55).
+// Measured: 4 x 2048 tokens of 8 heads of 128, turned, into 16-bit pages 15.0 us = 4.5 TB/s, ragged prompts of 6 sequences into 8-bit ones
+// 9.3; 64 single tokens in 8 bits 3.8-4.1 us, of which 3.3 are the host's; 8 sequences of up to 8192 tokens out of 8 bits 68 us = 5.4 TB/s
+// (a copy's rate: 6.55).
 #include <algorithm>
 
 #include <cuda_fp8.h>
@@ -341,7 +342,8 @@ int attn_b200_paged_append(const AttnB200PagedAppendArgs* a, void* cuda_stream) 
   p.rot = a->rotary;
   const int sms = device_sms();
   if (sms <= 0) return ATTN_B200_E_LAUNCH;
-  // heads are shared out evenly until two thirds of the chip's threads have work
+  // heads are shared out evenly until there is work for two thirds of the chip's threads; with 90 to 96 registers 640 of an SM's are
+  // resident at a time, so that a full call goes in up to 2.8 rounds of blocks (4 x 2048 tokens: 2048 blocks, 740 at a time)
   const long long one = rows * (a->cache.head_dim / 16), want = std::min<long long>(a->cache.heads_kv, (sms * 1365LL + one - 1) / one);
   const int rounds = static_cast<int>(a->cache.heads_kv / want);
   p.lanes = (a->cache.heads_kv + rounds - 1) / rounds;

@@ -13,11 +13,14 @@
 // The running maximum of a row is one value for a group, in the logarithm's scale; a tile is looked at for scores more than
 // 2^8 above it, by a barrier's reduction, and only then are maxima taken and the accumulator rescaled.  The sum of a row stays in
 // parts, one a thread, until the unit ends.
-// Measured: 64 sequences of up to 8192 tokens, 32 heads on 8 KV heads of 128: 206 us, 6.5 TB/s of the cache's bytes, the rate of a
-// copy.  8 bits, 16 sequences of up to 32768: 173 us, 4.3 TB/s: per tile of 128 rows (1130 ns) the widening of V and the softmax take
-// turns at the issue slots of twenty warps; a single sequence of 333 tokens 8.2 us, start, two tiles and end.
-// Units of 17 to 32 rows in 8 bits (32 rows of scores and sums in 96 registers): 16 sequences of 16384 tokens 164 us with 20 rows, 218 with
-// 32, where 16 rows take 141, and the same in 16 bits 168.
+// P is rounded to q's type, the operand's; its sum is taken of the unrounded values, in 32 bits.  (Error of o against 64 bits, relative
+// in the norm: 0.0023 in bf16 where the rounding of o alone gives 0.0017, as in the dense kernels.)
+// Measured: 64 sequences of up to 8192 tokens, 32 heads on 8 KV heads of 128: 209-212 us, 6.4 TB/s of the cache's bytes, 97 % of the rate
+// of a copy.  8 bits, 16 sequences of up to 32768: 178-184 us, 4.1 TB/s: per tile of 128 rows the widening of V and the softmax take
+// turns at the issue slots of twenty warps (54 % of them used, DRAM at 64 %); a single sequence of 333 tokens 8.2 us, start, three
+// tiles and end.
+// Units of 17 to 32 rows in 8 bits (32 rows of scores and sums in 96 registers, 208 bytes of spills a thread; 16 rows 12): 16 sequences of
+// 16384 tokens 163 us with 20 rows, 211-220 with 32, where 16 rows take 141, and 32 in 16 bits 172.
 #include <cstring>
 
 #include "paged_common.cuh"
@@ -341,7 +344,8 @@ paged_tokens_kernel(const __grid_constant__ PagedMaps maps, const __grid_constan
           }
         }
         // 16 rows in 8 bits hold their reference maxima and rescales (173 us for 182, 16 sequences of up to 32768); else they are read
-        // again where they are used: 32 rows in 8 bits spilled with them (298 us for 218, 16 sequences of 16384, 32 rows)
+        // again where they are used: 32 rows in 8 bits spilled more with them (298 us for 218, 16 sequences of 16384, 32 rows; 208 bytes
+        // a thread are left)
         constexpr bool kHold = k8Bit && R == 16;
         float ref[kHold ? R : 1], over = -INFINITY;
         auto hold = [&](int r, const float4& m) {

@@ -1,6 +1,6 @@
 // Rotary positions of q and k in one launch, forward and backward (the opposite angle): y = x with the first `dim` columns of
 // every head turned by position.  Bound by HBM: every value is read and written once.  4 x 4096 tokens of 40 heads of 128, there
-// and back: 121 us = 5.5 TB/s.
+// and back: 123 us = 5.5 TB/s; in 32 bits 217-222 us, 6.1 TB/s.
 //
 // A thread owns a unit of a token -- 16 bytes from each half of the turning columns, or 32 bytes of interleaved pairs -- and
 // walks the heads of q and k with it, so that the angles, cosines and sines of its pairs are made once for all heads and
