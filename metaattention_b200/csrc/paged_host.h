@@ -201,6 +201,8 @@ std::vector<Tensor> rotary_call(const std::shared_ptr<const Turns>& turns, const
   }
   for (const Tensor& t : x) {
     no_tangent("a rotation by positions", {&t});
+    for (int64_t d = 0; d < t.dim(); ++d)
+      if (t.size(d) > 0x7fffffff) refuse("up to 2^31 - 1 tokens, heads and columns are turned, got ", shape_of(t));
     has_memory("a tensor of heads", t);
     if (t.numel() > 0 && t.stride(-1) != 1) refuse("the last dimension must be contiguous");
   }

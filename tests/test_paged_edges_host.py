@@ -120,3 +120,12 @@ def test_tensors_without_memory_are_refused():
     for call in calls:
         with pytest.raises(ValueError, match="no memory"):
             call()
+
+
+def test_sizes_past_32_bits_are_refused():
+    """4294967301 tokens are not 5: the launch counts in 32 bits."""
+    row = torch.zeros(1, 1, 64)
+    for q, k in ((row.expand(2 ** 32 + 5, 1, 64), None), (row.expand(1, 2 ** 32 + 5, 64), None), (row, row.expand(1, 2 ** 31, 64)),
+                 (row.unsqueeze(0).expand(2 ** 31, 1, 1, 64), None)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            rotary(q, k, None, False)
